@@ -7,7 +7,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libfta.so")
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 FTA_F32, FTA_F16, FTA_BF16 = 0, 1, 2
 FTA_I32, FTA_I64 = 0, 1
 MASK_ADDITIVE_F32, MASK_PACKED_U64 = 0, 1
@@ -16,6 +16,7 @@ KERNEL_SHUFFLE, KERNEL_MFMA, KERNEL_MFMA_WIDE, KERNEL_MFMA_SPLIT_KEYS = 0, 1, 2,
 EXPORTED_SYMBOLS = (
     "fta_abi_version", "fta_strerror", "fta_validate", "fta_plan", "fta_decode", "fta_decode_stage1",
     "fta_decode_stage2", "fta_device_cus", "fta_append_kv",
+    "fta_rotary", "fta_logprobs_workspace", "fta_logprobs", "fta_accept_path",
 )
 
 # status -> Python exception class
@@ -50,6 +51,39 @@ class FtaAppendArgs(C.Structure):
         ("page_size", C.c_int32), ("reserved", C.c_int32),
         ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("ck_stride", C.c_int64 * 3), ("cv_stride", C.c_int64 * 3),
         ("accept_idx_stride", C.c_int64), ("block_table_stride", C.c_int64),
+    ]
+
+
+class FtaRotaryArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("out_q", C.c_void_p), ("out_k", C.c_void_p),
+        ("positions", C.c_void_p), ("kv_seq_len", C.c_void_p), ("inv_freq", C.c_void_p),
+        ("bsz", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("q_len", C.c_int32),
+        ("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("dtype", C.c_int32), ("pos_dtype", C.c_int32),
+        ("len_dtype", C.c_int32), ("freq_is_f64", C.c_int32), ("interleaved", C.c_int32), ("inverse", C.c_int32),
+        ("attention_factor", C.c_float), ("reserved", C.c_int32),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("out_q_stride", C.c_int64 * 3),
+        ("out_k_stride", C.c_int64 * 3), ("pos_stride", C.c_int64 * 2),
+    ]
+
+
+class FtaLogprobArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("token_ids", C.c_void_p), ("logprobs", C.c_void_p), ("entropy", C.c_void_p),
+        ("lse", C.c_void_p), ("top_logprobs", C.c_void_p), ("top_ids", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int32), ("num_ids", C.c_int32),
+        ("top_k", C.c_int32), ("dtype", C.c_int32), ("id_dtype", C.c_int32), ("inv_temperature", C.c_float),
+        ("logits_stride", C.c_int64), ("id_stride", C.c_int64 * 2),
+    ]
+
+
+class FtaAcceptArgs(C.Structure):
+    _fields_ = [
+        ("tree_tokens", C.c_void_p), ("target_tokens", C.c_void_p), ("parents", C.c_void_p), ("accept_idx", C.c_void_p),
+        ("accept_len", C.c_void_p), ("next_token", C.c_void_p),
+        ("bsz", C.c_int32), ("q_len", C.c_int32), ("max_accept", C.c_int32), ("token_dtype", C.c_int32),
+        ("target_dtype", C.c_int32), ("parent_dtype", C.c_int32), ("len_dtype", C.c_int32), ("reserved", C.c_int32),
+        ("token_stride", C.c_int64 * 2), ("target_stride", C.c_int64 * 2), ("parent_stride", C.c_int64 * 2),
     ]
 
 
@@ -109,6 +143,12 @@ def load() -> C.CDLL:
     lib.fta_device_cus.restype = C.c_int
     lib.fta_append_kv.restype = C.c_int
     lib.fta_append_kv.argtypes = [C.POINTER(FtaAppendArgs), C.c_void_p]
+    for name, args in (("fta_rotary", FtaRotaryArgs), ("fta_logprobs", FtaLogprobArgs), ("fta_accept_path", FtaAcceptArgs)):
+        fn = getattr(lib, name)
+        fn.restype = C.c_int
+        fn.argtypes = [C.POINTER(args), C.c_void_p]
+    lib.fta_logprobs_workspace.restype = C.c_int
+    lib.fta_logprobs_workspace.argtypes = [C.POINTER(FtaLogprobArgs), C.POINTER(C.c_int64)]
     if lib.fta_abi_version() != ABI_VERSION:
         raise ImportError(f"libfta.so has ABI {lib.fta_abi_version()}, binding expects {ABI_VERSION}; rebuild it")
     _lib = lib

@@ -14,7 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB_PATH = os.path.join(HERE, "libfta.so")
-SOURCES = ["fta_host.cpp", "stage1_shuffle.hip", "stage1_mfma.hip", "stage1_mfma_wide.hip", "stage1_mfma_splitkeys.hip", "stage2_merge.hip", "append_kv.hip"]
+SOURCES = ["fta_host.cpp", "stage1_shuffle.hip", "stage1_mfma.hip", "stage1_mfma_wide.hip", "stage1_mfma_splitkeys.hip", "stage2_merge.hip", "append_kv.hip",
+           "rotary.hip", "token_logprobs.hip", "accept_path.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
@@ -25,13 +26,15 @@ FLAGS = [
     "-fno-honor-nans",
     "-I", INCLUDE, "-I", CSRC,
 ] + os.environ.get("FTA_EXTRA_FLAGS", "").split()
+# Sources that give NaN a meaning of its own (a NaN logit makes its row's results NaN).
+SOURCE_FLAGS = {"token_logprobs.hip": ["-fhonor-nans"]}
 
 
 def _compile(src: str) -> str:
     obj_dir = os.path.join(HERE, "build")
     os.makedirs(obj_dir, exist_ok=True)
     obj = os.path.join(obj_dir, os.path.splitext(src)[0] + ".o")
-    cmd = [HIPCC, *FLAGS, "-x", "hip", "-c", os.path.join(CSRC, src), "-o", obj]
+    cmd = [HIPCC, *FLAGS, *SOURCE_FLAGS.get(src, []), "-x", "hip", "-c", os.path.join(CSRC, src), "-o", obj]
     res = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in res.stderr.splitlines() if noise not in l)

@@ -76,6 +76,18 @@ def accepted_paths(parents: Sequence[int], nodes: Sequence[int], device=None):
     return (idx.to(device), lens.to(device)) if device is not None else (idx, lens)
 
 
+def tree_depths(parents: Sequence[int], device=None) -> torch.Tensor:
+    """int32 [L]: edges between every node and its root (0 at a root), the node's position behind the cached keys."""
+    p = [int(x) for x in parents]
+    depth = []
+    for i, j in enumerate(p):
+        if not (-1 <= j < i):
+            raise ValueError(f"parent[{i}] = {j} is not in [-1, {i})")
+        depth.append(depth[j] + 1 if j >= 0 else 0)
+    d = torch.tensor(depth, dtype=torch.int32)
+    return d.to(device) if device is not None else d
+
+
 def ancestor_matrix(parents: Sequence[int]) -> torch.Tensor:
     """Boolean [L, L]: entry (i, j) is True iff j is i or an ancestor of i. Parents
     must precede their children (parent[i] < i), roots carry -1."""

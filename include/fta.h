@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define FTA_ABI_VERSION 3
+#define FTA_ABI_VERSION 4
 
 typedef enum fta_status {
   FTA_OK = 0,
@@ -259,6 +259,123 @@ typedef struct fta_append_args {
 
 /* Validates, then launches on `hip_stream`. Asynchronous; allocates nothing. */
 int fta_append_kv(const fta_append_args* args, void* hip_stream);
+
+/*
+ * Rotary positions for the rows that enter a tree-attention call. Row i of sequence b stands at
+ *     pos = positions[b, i] + (kv_seq_len ? kv_seq_len[b] : 0)
+ * (tree rows: positions = depth in the tree, kv_seq_len = keys in front of the tree), and the first
+ * rotary_dim values of every head are turned in pairs: with a = pos * inv_freq[t], negated for `inverse`,
+ *     (x, y) -> attention_factor * (x cos a - y sin a, y cos a + x sin a)
+ * Pair t is (t, t + rotary_dim / 2), or (2t, 2t + 1) with `interleaved`. Values from rotary_dim on are
+ * copied unchanged. Angles are taken in 64 bits, values in 32, each result is rounded once.
+ * out_q / out_k may be q / k themselves (in place); any other overlap is the caller's error. k and out_k may
+ * both be NULL. Strides in elements, inner stride 1, rows 16-byte aligned.
+ */
+typedef struct fta_rotary_args {
+  const void* q;             /* [bsz, num_q_heads, q_len, head_dim] */
+  const void* k;             /* [bsz, num_kv_heads, q_len, head_dim], or NULL */
+  void* out_q;
+  void* out_k;
+  const void* positions;     /* [bsz or 1, q_len], pos_dtype */
+  const void* kv_seq_len;    /* [bsz], len_dtype, or NULL */
+  const void* inv_freq;      /* [rotary_dim / 2], float64 or float32 (freq_is_f64), radians per position */
+
+  int32_t bsz;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;      /* 0 when k is NULL */
+  int32_t q_len;
+  int32_t head_dim;          /* 32, 64, 128 or 256 */
+  int32_t rotary_dim;        /* even, 2 .. head_dim */
+  int32_t dtype;             /* fta_dtype */
+  int32_t pos_dtype;         /* fta_len_dtype of positions */
+  int32_t len_dtype;         /* fta_len_dtype of kv_seq_len */
+  int32_t freq_is_f64;
+  int32_t interleaved;
+  int32_t inverse;
+  float attention_factor;
+  int32_t reserved;
+
+  int64_t q_stride[3];       /* batch, head, row */
+  int64_t k_stride[3];
+  int64_t out_q_stride[3];
+  int64_t out_k_stride[3];
+  int64_t pos_stride[2];     /* batch (0 = the same row of positions for every sequence), row */
+} fta_rotary_args;
+
+/* Validates, then launches on `hip_stream`. Asynchronous; allocates nothing. */
+int fta_rotary(const fta_rotary_args* args, void* hip_stream);
+
+/*
+ * Log probabilities of given tokens, entropy and the largest alternatives, from rows of logits. With
+ * y = logits * inv_temperature and lse = log sum exp y over the vocabulary:
+ *     logprobs[r, j] = y[token_ids[r, j]] - lse[r]     (-inf where the id is outside [0, vocab))
+ *     entropy[r]     = lse - sum p y,  p = exp(y - lse) (a logit of -inf adds nothing)
+ *     top_ids[r, :]  = the top_k largest logits, descending, equal logits by ascending id
+ *     top_logprobs   = their log probabilities
+ * A row whose every logit is -inf has lse = -inf, entropy 0 and log probabilities of -inf. A NaN or +inf in a
+ * row makes its lse, entropy and log probabilities NaN (among the alternatives NaN counts as less than
+ * -inf). All sums in 32 bits; outputs are float32 / int64.
+ */
+typedef struct fta_logprob_args {
+  const void* logits;        /* [rows, vocab], row stride logits_stride, inner stride 1, any alignment of its type */
+  const void* token_ids;     /* [rows, num_ids], id_dtype, or NULL when num_ids is 0 */
+  float* logprobs;           /* [rows, num_ids] dense, or NULL when num_ids is 0 */
+  float* entropy;            /* [rows] */
+  float* lse;                /* [rows] */
+  float* top_logprobs;       /* [rows, top_k] dense, or NULL when top_k is 0 */
+  int64_t* top_ids;          /* [rows, top_k] dense, or NULL when top_k is 0 */
+  void* workspace;           /* fta_logprobs_workspace() bytes, 16-byte aligned; NULL when that is 0 */
+
+  int64_t workspace_bytes;
+  int64_t rows;
+  int32_t vocab;
+  int32_t num_ids;
+  int32_t top_k;             /* 0 .. min(vocab, 128) */
+  int32_t dtype;             /* fta_dtype of logits */
+  int32_t id_dtype;          /* fta_len_dtype of token_ids */
+  float inv_temperature;     /* > 0 */
+  int64_t logits_stride;
+  int64_t id_stride[2];      /* row, column of token_ids */
+} fta_logprob_args;
+
+/* Writes the bytes of workspace that fta_logprobs needs for these sizes (0 for none). Pure host code; judges the
+ * sizes only, so the pointers may still be NULL. */
+int fta_logprobs_workspace(const fta_logprob_args* args, int64_t* bytes);
+/* Validates, then launches on `hip_stream`. Asynchronous; allocates nothing. */
+int fta_logprobs(const fta_logprob_args* args, void* hip_stream);
+
+/*
+ * The accepted path of a draft tree. Node 0 (the root: the last token that is certain) is always accepted;
+ * from an accepted node c the path goes on to the first node i (in index order) with parents[i] == c and
+ * tree_tokens[i] == target_tokens[c], until there is none or max_accept nodes are taken.
+ *     accept_idx[b, 0 .. accept_len[b])  the path's nodes, root first (0 behind it): what fta_append_kv takes
+ *     next_token[b]                      target_tokens at the path's last node: the token that follows it
+ * Parents precede their children; a node i > 0 whose parent is not in [0, i) hangs nowhere (padding of a
+ * batch of trees) and is never accepted.
+ */
+typedef struct fta_accept_args {
+  const void* tree_tokens;   /* [bsz, q_len], token_dtype */
+  const void* target_tokens; /* [bsz, q_len], target_dtype: the token the model picks after each node */
+  const void* parents;       /* [bsz or 1, q_len], parent_dtype */
+  int32_t* accept_idx;       /* [bsz, max_accept] dense */
+  void* accept_len;          /* [bsz], len_dtype */
+  void* next_token;          /* [bsz], target_dtype */
+
+  int32_t bsz;
+  int32_t q_len;             /* 1 .. 16384 */
+  int32_t max_accept;        /* >= 1 */
+  int32_t token_dtype;       /* fta_len_dtype */
+  int32_t target_dtype;      /* fta_len_dtype */
+  int32_t parent_dtype;      /* fta_len_dtype */
+  int32_t len_dtype;         /* fta_len_dtype of accept_len */
+  int32_t reserved;
+  int64_t token_stride[2];   /* batch, node */
+  int64_t target_stride[2];
+  int64_t parent_stride[2];  /* batch (0 = one tree for all), node */
+} fta_accept_args;
+
+/* Validates, then launches on `hip_stream`. Asynchronous; allocates nothing. */
+int fta_accept_path(const fta_accept_args* args, void* hip_stream);
 
 /* Number of compute units of the current HIP device, or a negative fta_status. */
 int fta_device_cus(void);
