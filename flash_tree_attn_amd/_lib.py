@@ -17,6 +17,7 @@ EXPORTED_SYMBOLS = (
     "fta_abi_version", "fta_strerror", "fta_validate", "fta_plan", "fta_decode", "fta_decode_stage1",
     "fta_decode_stage2", "fta_device_cus", "fta_append_kv",
     "fta_rotary", "fta_logprobs_workspace", "fta_logprobs", "fta_accept_path",
+    "fta_shaped_workspace", "fta_shaped_decode",
 )
 
 # status -> Python exception class
@@ -87,6 +88,21 @@ class FtaAcceptArgs(C.Structure):
     ]
 
 
+class FtaShapedArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("cur_k", C.c_void_p), ("cur_v", C.c_void_p),
+        ("mask", C.c_void_p), ("kv_seq_len", C.c_void_p), ("out", C.c_void_p), ("block_table", C.c_void_p),
+        ("slopes", C.c_void_p), ("first_key", C.c_void_p), ("depths", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64), ("bsz", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32),
+        ("cur_heads", C.c_int32), ("q_len", C.c_int32), ("head_dim", C.c_int32), ("cache_len", C.c_int32),
+        ("max_seq_len_hint", C.c_int32), ("page_size", C.c_int32), ("dtype", C.c_int32), ("len_dtype", C.c_int32),
+        ("mask_kind", C.c_int32), ("window", C.c_int32), ("softcap", C.c_float), ("sm_scale", C.c_float), ("reserved", C.c_int32),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("ck_stride", C.c_int64 * 3),
+        ("cv_stride", C.c_int64 * 3), ("mask_stride", C.c_int64 * 3), ("out_stride", C.c_int64 * 3),
+        ("block_table_stride", C.c_int64), ("depth_stride", C.c_int64),
+    ]
+
+
 LEN_BUCKETS = 16   # FTA_LEN_BUCKETS
 
 
@@ -143,12 +159,15 @@ def load() -> C.CDLL:
     lib.fta_device_cus.restype = C.c_int
     lib.fta_append_kv.restype = C.c_int
     lib.fta_append_kv.argtypes = [C.POINTER(FtaAppendArgs), C.c_void_p]
-    for name, args in (("fta_rotary", FtaRotaryArgs), ("fta_logprobs", FtaLogprobArgs), ("fta_accept_path", FtaAcceptArgs)):
+    for name, args in (("fta_rotary", FtaRotaryArgs), ("fta_logprobs", FtaLogprobArgs), ("fta_accept_path", FtaAcceptArgs),
+                       ("fta_shaped_decode", FtaShapedArgs)):
         fn = getattr(lib, name)
         fn.restype = C.c_int
         fn.argtypes = [C.POINTER(args), C.c_void_p]
     lib.fta_logprobs_workspace.restype = C.c_int
     lib.fta_logprobs_workspace.argtypes = [C.POINTER(FtaLogprobArgs), C.POINTER(C.c_int64)]
+    lib.fta_shaped_workspace.restype = C.c_int
+    lib.fta_shaped_workspace.argtypes = [C.POINTER(FtaShapedArgs), C.c_int, C.POINTER(C.c_int64)]
     if lib.fta_abi_version() != ABI_VERSION:
         raise ImportError(f"libfta.so has ABI {lib.fta_abi_version()}, binding expects {ABI_VERSION}; rebuild it")
     _lib = lib

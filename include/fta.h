@@ -377,6 +377,70 @@ typedef struct fta_accept_args {
 /* Validates, then launches on `hip_stream`. Asynchronous; allocates nothing. */
 int fta_accept_path(const fta_accept_args* args, void* hip_stream);
 
+/*
+ * Tree attention with shaped scores. As fta_decode, but the score of query row i (at position p_i = T_b +
+ * depths[b, i], T_b = kv_seq_len[b]) and a key at position p_j (a cache key j stands at j, tree key j at
+ * T_b + depths[b, j]) is
+ *     x = sm_scale q_i . k_j
+ *     y = softcap > 0 ? softcap * tanh(x / softcap) : x
+ *     z = y - slopes[head] * (p_i - p_j)  [+ mask[i, j] for a tree key]
+ * and a key is left out where p_i - p_j >= window (window > 0), a cache key also where j < first_key[b] (the
+ * start of this sequence's document in its cache row). A row that sees nothing yields zeros. Cache rows that no
+ * query of the call may see are not read; a value row that none of the rows of a wave (32 query rows) sees adds
+ * nothing whatever it holds. Additive mask values below -2.3e38 that are not -inf count as that value.
+ * Everything else (shapes, strides, paged caches, mask kinds, length types) is as in fta_args, for float32 too.
+ */
+typedef struct fta_shaped_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const void* cur_k;
+  const void* cur_v;
+  const void* mask;
+  const void* kv_seq_len;
+  void* out;
+  const int32_t* block_table; /* NULL = contiguous caches */
+  const float* slopes;        /* [num_q_heads], or NULL */
+  const int32_t* first_key;   /* [bsz], clamped to [0, kv_seq_len], or NULL = 0 */
+  const int32_t* depths;      /* [bsz or 1, q_len], negative ones count as 0; NULL = 0, 1, 2, ... (a chain) */
+  void* workspace;            /* fta_shaped_workspace() bytes, 16-byte aligned; NULL when that is 0 */
+
+  int64_t workspace_bytes;
+  int32_t bsz;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t cur_heads;          /* num_kv_heads or num_q_heads */
+  int32_t q_len;
+  int32_t head_dim;
+  int32_t cache_len;
+  int32_t max_seq_len_hint;   /* an upper bound of kv_seq_len, 0 = cache_len; sizes the launch only */
+  int32_t page_size;
+  int32_t dtype;
+  int32_t len_dtype;
+  int32_t mask_kind;
+  int32_t window;             /* 0 = none */
+  float softcap;              /* 0 = none */
+  float sm_scale;             /* any sign */
+  int32_t reserved;
+
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t ck_stride[3];
+  int64_t cv_stride[3];
+  int64_t mask_stride[3];
+  int64_t out_stride[3];
+  int64_t block_table_stride;
+  int64_t depth_stride;       /* batch stride of depths, 0 = the same tree for every sequence */
+} fta_shaped_args;
+
+/* Writes the bytes of workspace that fta_shaped_decode needs on a device of num_cus compute units (0 = 256; 0 bytes
+ * where it needs none). Pure host code; judges the sizes only. */
+int fta_shaped_workspace(const fta_shaped_args* args, int num_cus, int64_t* bytes);
+/* Validates, then launches on `hip_stream` (one kernel, or two where sequences are cut). Asynchronous; allocates
+ * nothing. The workspace may hold anything; calls that may overlap in time need workspaces of their own. */
+int fta_shaped_decode(const fta_shaped_args* args, void* hip_stream);
+
 /* Number of compute units of the current HIP device, or a negative fta_status. */
 int fta_device_cus(void);
 

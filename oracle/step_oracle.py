@@ -102,7 +102,7 @@ def shaped_attention_oracle(q, k_cache, v_cache, current_k, current_v, mask, kv_
                 z = softcap * torch.tanh(z / softcap)
             if slopes is not None:
                 z = z - float(slopes[h]) * away
-            z[:, T - first:] += mask[b, h]
+            z[:, T - first:] = torch.where(mask[b, h] == float("-inf"), float("-inf"), z[:, T - first:] + mask[b, h])
             if window:
                 z = z.masked_fill(away >= window, float("-inf"))
             top = z.amax(-1, keepdim=True)
