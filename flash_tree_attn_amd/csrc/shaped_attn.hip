@@ -47,6 +47,7 @@ struct ShapedParams {
   int32_t rows, row_blocks, groups, tree_tiles;   // groups: stretches per row block
   int32_t whole;          // every (sequence, unit) pair is a stretch of its own
   int32_t rows_cap;       // rows per partial
+  int32_t lead_groups, lead_permille;   // the first lead_groups stretches hold lead_permille / 1000 of the line; 0: all alike
   int32_t len_is_i64, mask_packed, page_shift, window;
   float scale, softcap;
   int64_t partial_floats; // per partial
@@ -59,6 +60,9 @@ struct ShapedParams {
 constexpr int kTreeWeight = 3;
 // Stretches are at least this many tiles long: below, the prologue and the partials cost more than they spread.
 constexpr int kMinStretch = 4;
+
+// 2^z is 0 in 32 bits for z up to here (the smallest positive value is 2^-149).
+constexpr float kNoWeight = -150.f;
 
 // One 1 KiB block of LDS per wave-wide load: 1024 / ROW_BYTES rows, their 16-byte chunks interleaved, blocks 1024 +
 // one chunk column apart, so that both operand reads fall on distinct banks and every fragment address is a lane
@@ -121,50 +125,72 @@ __device__ __forceinline__ Sequence sequence_of(const ShapedParams& p, int b) {
   s.n = s.n_cache + kTreeWeight * p.tree_tiles;
   return s;
 }
-// Sums over the sequences in front of `until` and over all of them, of their stretch per unit. Every lane of the
-// wave must call it.
-template <int KEYS>
-__device__ __forceinline__ void line_sums(const ShapedParams& p, int until, int* before, int* total) {
+// The line: every sequence's units, one after the other. Each lane of a wave looks at one sequence of a batch of up to
+// 64; larger batches in rounds.
+struct Place {
+  int b;       // sequence
+  int begin;   // where its first unit begins
+  int total;   // length of the whole line
+  Sequence seq;
+};
+// The place of x = at(total) on the line, for the kernel, or (with by_sequence) of sequence `at` itself, for the join.
+// Every lane of the wave must call it.
+template <int KEYS, typename At>
+__device__ __forceinline__ Place place_of(const ShapedParams& p, bool by_sequence, At&& at) {
   const int lane = threadIdx.x & 63;
-  int part = 0, all = 0;
-  for (int c = 0; c < p.bsz; c += 64) {
-    const int n = c + lane < p.bsz ? sequence_of<KEYS>(p, c + lane).n : 0;
-    all += n;
-    part += c + lane < until ? n : 0;
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    all += __shfl_xor(all, o, 64);
-    part += __shfl_xor(part, o, 64);
-  }
-  *total = __builtin_amdgcn_readfirstlane(all);
-  *before = __builtin_amdgcn_readfirstlane(part);
-}
-// The sequence that holds place x of the line, and where its part begins. Every lane of the wave must call it.
-template <int KEYS>
-__device__ __forceinline__ int sequence_at(const ShapedParams& p, int x, int* begin) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int c = 0; c < p.bsz; c += 64) {
-    const int n = (c + lane < p.bsz ? sequence_of<KEYS>(p, c + lane).n : 0) * p.units;
-    int upto = n;   // inclusive scan
+  Place r{-1, 0, 0, {}};
+  Sequence mine{};
+  int n = 0, upto = 0;   // of this lane's sequence: its length on the line, and that of all up to it in this round
+  auto look = [&](int c) __attribute__((always_inline)) {
+    mine = sequence_of<KEYS>(p, min(c + lane, p.bsz - 1));
+    n = c + lane < p.bsz ? mine.n * p.units : 0;
+    upto = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int y = __shfl_up(upto, o, 64);
       upto += lane >= o ? y : 0;
     }
-    const uint64_t holds = __builtin_amdgcn_ballot_w64(n > 0 && x < base + upto);
+    return __builtin_amdgcn_readlane(upto, 63);
+  };
+  for (int c = 0; c < p.bsz; c += 64) r.total += look(c);
+  const int x = at(r.total);
+  int base = 0;
+  for (int c = 0; c < p.bsz; c += 64) {
+    const int round = p.bsz > 64 ? look(c) : r.total;
+    const uint64_t holds = __builtin_amdgcn_ballot_w64(by_sequence ? c + lane == x : n > 0 && x < base + upto);
     if (holds) {
       const int l = __builtin_ctzll(holds);
-      *begin = base + __builtin_amdgcn_readlane(upto - n, l);
-      return c + l;
+      r.b = c + l;
+      r.begin = base + __builtin_amdgcn_readlane(upto - n, l);
+      r.seq.length = __builtin_amdgcn_readlane(mine.length, l);
+      r.seq.first = __builtin_amdgcn_readlane(mine.first, l);
+      r.seq.lo = __builtin_amdgcn_readlane(mine.lo, l);
+      r.seq.tile0 = __builtin_amdgcn_readlane(mine.tile0, l);
+      r.seq.n_cache = __builtin_amdgcn_readlane(mine.n_cache, l);
+      r.seq.n = __builtin_amdgcn_readlane(mine.n, l);
+      return r;
     }
-    base += __builtin_amdgcn_readlane(upto, 63);
+    base += round;
   }
-  return -1;
+  return r;
 }
-__device__ __forceinline__ int stretch_of(const ShapedParams& p, int per_unit_total) {
-  return max((per_unit_total * p.units + p.groups - 1) / p.groups, kMinStretch);
+
+// How the line is cut: `heads` stretches of `lead` places, then stretches of `tail`.
+struct Stretches {
+  int heads, lead, tail;
+  __device__ __forceinline__ int start(int g) const { return g < heads ? g * lead : heads * lead + (g - heads) * tail; }
+  __device__ __forceinline__ int holder(int x) const { return x < heads * lead ? x / lead : heads + (x - heads * lead) / tail; }
+};
+__device__ __forceinline__ Stretches cut_line(const ShapedParams& p, int total) {
+  Stretches s;
+  const int even = max((total + p.groups - 1) / p.groups, kMinStretch);
+  s.heads = p.lead_groups;
+  s.lead = s.tail = even;
+  if (p.lead_groups > 0 && even > 2 * kMinStretch) {
+    s.lead = static_cast<int>((static_cast<int64_t>(total) * p.lead_permille + 1000 * p.lead_groups - 1) / (1000 * p.lead_groups));
+    s.tail = max((total - s.lead * s.heads + p.groups - s.heads - 1) / (p.groups - s.heads), kMinStretch);
+  }
+  return s;
 }
 
 template <typename T, int D, int WK, bool PAGED>
@@ -215,23 +241,28 @@ shaped_kernel(const ShapedParams p) {
     begin = x0 = x = 0;
     x1 = seq.n;
   } else {
-    int total, before;
-    line_sums<kKeys>(p, 0, &before, &total);
-    const int stretch = stretch_of(p, total);
-    total *= p.units;
-    if (group > (total - 1) / stretch) return;
-    x0 = x = group * stretch;
-    x1 = min(x0 + stretch, total);
-    b = sequence_at<kKeys>(p, x0, &begin);
-    seq = sequence_of<kKeys>(p, b);
-    unit = (x0 - begin) / seq.n;
-    begin += unit * seq.n;
+    bool none = false;
+    const Place here = place_of<kKeys>(p, false, [&](int total) __attribute__((always_inline)) {
+      const Stretches cut = cut_line(p, total);
+      x0 = cut.start(group);
+      x1 = min(cut.start(group + 1), total);
+      none = x0 >= total;
+      return min(x0, total - 1);
+    });
+    if (none) return;
+    x = x0;
+    b = here.b;
+    seq = here.seq;
+    unit = (x0 - here.begin) / seq.n;
+    begin = here.begin + unit * seq.n;
   }
 
   // ---- lane constants of the loads and of the operand reads
   const int ld_row = lane % RPB, ld_chunk = lane / RPB;   // lane i fetches chunk i / RPB of row i % RPB of a block
   const int64_t k_row = p.k_stride[2] * ES, v_row = p.v_stride[2] * ES;
-  const uint32_t k_lane = static_cast<uint32_t>(ld_row * k_row + ld_chunk * 16), v_lane = static_cast<uint32_t>(ld_row * v_row + ld_chunk * 16);
+  // bytes from a tile's first row to this lane's piece of its block (of its wave's first block, for contiguous caches)
+  const int64_t k_lane = ((PAGED ? 0 : wave * RPB) + ld_row) * k_row + ld_chunk * 16, v_lane = ((PAGED ? 0 : wave * RPB) + ld_row) * v_row + ld_chunk * 16;
+  const int64_t k_step = 4 * RPB * k_row, v_step = 4 * RPB * v_row;   // to the wave's next block
   const uint32_t lds0 = lds_address(smem);
   const int kb0 = WK == 2 ? (wave & 1) * NB : 0;          // first key block of this wave
   const uint32_t k_rd = lds0 + Tile::at(li, lh) + kb0 * Tile::at(32, 0);
@@ -243,13 +274,12 @@ shaped_kernel(const ShapedParams p) {
   const int page_mask = (1 << p.page_shift) - 1;
   const int64_t k_page = p.k_stride[0] * ES, v_page = p.v_stride[0] * ES;
 
-  // scores in units of log2 e: no cap z = c s; with one z = cap2 - 2 cap2 / (1 + 2^(ex s)), the tanh written out
-  const bool capped = p.softcap > 0.f;
+  // Scores in units of log2 e: without a cap z = c s; with one cap2 tanh(x / cap), the tanh written out as
+  // 1 - 2 / (1 + 2^(ex s)) (f32: taken as it is, of ex s).
+  const bool capped = p.softcap > 0.f, sloped = p.slopes != nullptr;
   const float c = p.scale * kLog2e;
   const float cap2 = p.softcap * kLog2e;
-  const float ex = capped ? 2.f * kLog2e * p.scale / p.softcap : 0.f;
-  // Full tiles of calls without a bias take the row maximum from the raw products, which needs a growing shape.
-  const bool growing = p.scale > 0.f && !p.slopes;
+  const float ex = capped ? (kIs32<T> ? 1.f : 2.f * kLog2e) * p.scale / p.softcap : 0.f;
 
   for (;;) {
     // ---- one pair: places [from, to) of its stretch
@@ -258,7 +288,10 @@ shaped_kernel(const ShapedParams p) {
     const int cache_from = min(from, seq.n_cache), cache_tiles = min(to, seq.n_cache) - cache_from;
     const int u0 = (max(from - seq.n_cache, 0) + kTreeWeight - 1) / kTreeWeight;   // tree tiles whose first place is in [from, to)
     const int u1 = to > seq.n_cache ? (to - seq.n_cache + kTreeWeight - 1) / kTreeWeight : 0;
-    const int tiles = cache_tiles + max(u1 - u0, 0);
+    // Nearest keys first: the tree's tiles, then the cache's from the last one back, so that with a bias the running
+    // maximum is there at once and what follows only falls.
+    const int trees = max(u1 - u0, 0), tiles = trees + cache_tiles;
+    const int last_tile = seq.tile0 + cache_from + cache_tiles - 1;
     const int T_b = seq.length;
 
     const int head0 = unit * p.heads_per_unit;
@@ -267,13 +300,13 @@ shaped_kernel(const ShapedParams p) {
     const char* vbase = static_cast<const char*>(p.v) + ((PAGED ? 0 : b * p.v_stride[0]) + cache_head * p.v_stride[1]) * ES;
     const int32_t* table = PAGED ? p.table + b * p.table_stride : nullptr;
 
-    // pages of the blocks of the next full tile, requested when the tile in front of it goes out
+    // pages of the blocks of the next cache tile, requested when the one ahead of it goes out
     int page_of[kLoads];
     auto look_up = [&](int tile) __attribute__((always_inline)) {
       if constexpr (PAGED) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-          const int key = min(tile * kKeys + (i * 4 + wave) * RPB, p.cache_len - 1);
+          const int key = min(max(tile, 0) * kKeys + (i * 4 + wave) * RPB, p.cache_len - 1);
           page_of[i] = load_uniform(table + (key >> p.page_shift));
         }
       }
@@ -301,36 +334,40 @@ shaped_kernel(const ShapedParams p) {
     auto request_tree = [&](int t) __attribute__((always_inline)) {
       const auto* c = parameters_again(p);
       const int cur_head = unit * c->heads_per_unit / c->cur_group;
-      request_rows(std::true_type{}, t, (u0 + t - cache_tiles) * kKeys, static_cast<const char*>(c->ck) + (b * c->ck_stride[0] + cur_head * c->ck_stride[1]) * ES,
+      request_rows(std::true_type{}, t, (u0 + t) * kKeys, static_cast<const char*>(c->ck) + (b * c->ck_stride[0] + cur_head * c->ck_stride[1]) * ES,
                    static_cast<const char*>(c->cv) + (b * c->cv_stride[0] + cur_head * c->cv_stride[1]) * ES, c->ck_stride[2] * ES, c->cv_stride[2] * ES, 0, L - 1);
     };
     auto request = [&](int t) __attribute__((always_inline)) {
-      if (t >= cache_tiles) {
+      if (t < trees) {
         request_tree(t);
         return;
       }
-      const int tile = seq.tile0 + cache_from + t, key0 = tile * kKeys;
+      const int tile = last_tile - (t - trees), key0 = tile * kKeys;
       if (key0 >= seq.lo && key0 + kKeys <= T_b) {
         char* kst = smem + (t % kStages) * Tile::kBytes;
         char* vst = kst + kVRing;
+        if constexpr (PAGED) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int blk = i * 4 + wave;
-          const int key = key0 + blk * RPB;
-          int64_t koff = key * k_row, voff = key * v_row;
-          if constexpr (PAGED) {
-            koff = page_of[i] * k_page + (key & page_mask) * k_row;
-            voff = page_of[i] * v_page + (key & page_mask) * v_row;
+          for (int i = 0; i < kLoads; ++i) {
+            const int blk = i * 4 + wave, at = (key0 + blk * RPB) & page_mask;
+            FTA_LOAD_BLOCK_TO_LDS(kbase + (page_of[i] * k_page + at * k_row) + k_lane, kst + blk * Tile::kBlockPitch);
+            FTA_LOAD_BLOCK_TO_LDS(vbase + (page_of[i] * v_page + at * v_row) + v_lane, vst + blk * Tile::kBlockPitch);
           }
-          FTA_LOAD_BLOCK_TO_LDS(uniform_ptr(kbase + koff) + k_lane, kst + blk * Tile::kBlockPitch);
-          FTA_LOAD_BLOCK_TO_LDS(uniform_ptr(vbase + voff) + v_lane, vst + blk * Tile::kBlockPitch);
+        } else {
+          const char* ksrc = kbase + key0 * k_row + k_lane;
+          const char* vsrc = vbase + key0 * v_row + v_lane;
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            FTA_LOAD_BLOCK_TO_LDS(ksrc + i * k_step, kst + (i * 4 + wave) * Tile::kBlockPitch);
+            FTA_LOAD_BLOCK_TO_LDS(vsrc + i * v_step, vst + (i * 4 + wave) * Tile::kBlockPitch);
+          }
         }
       } else {
         request_rows(std::false_type{}, t, key0, kbase, vbase, k_row, v_row, seq.lo, T_b - 1);
       }
-      look_up(tile + 1);
+      look_up(tile - 1);
     };
-    if (cache_tiles > 0) look_up(seq.tile0 + cache_from);
+    if (cache_tiles > 0) look_up(last_tile);
     if (tiles > 0) request(0);
 
     // ---- this lane's query row
@@ -450,11 +487,17 @@ shaped_kernel(const ShapedParams p) {
       wait_vmcnt<0>();          // this wave's part of tile t has landed ...
       workgroup_barrier();      // ... and everybody's, and everybody is done with tile t - 1, whose stage tile t + 1 takes
       if (t + 1 < tiles) request(t + 1);
-      const bool tree = t >= cache_tiles;
+      const bool tree = t < trees;
       if (!wave_active && !tree) continue;
       const uint32_t stage = (t % kStages) * Tile::kBytes;
-      const int key0 = (tree ? u0 + t - cache_tiles : seq.tile0 + cache_from + t) * kKeys;
+      const int key0 = (tree ? u0 + t : last_tile - (t - trees)) * kKeys;
       const int lane_key = key0 + lane_key0;
+      // A tile whose capped scores, lowered by their distance, are all more than 2^150 below the row's maximum has
+      // weights of exactly 0 in 32 bits: nothing of it would be added.
+      if (capped && sloped && !tree) {
+        const float nearest = static_cast<float>(pos - key0 - (kKeys - 1)), farthest = static_cast<float>(pos - key0);
+        if (!wave_any(row_ok && !(cap2 - fminf(slope * nearest, slope * farthest) < m_run + kNoWeight))) continue;
+      }
 
       // ---- S^T = K Q^T, fragments requested a few products ahead
       float s[NB][16];
@@ -467,6 +510,7 @@ shaped_kernel(const ShapedParams p) {
           constexpr int F = decltype(f)::value;
           kf[F] = lds_read_b128<(F % NB) * Tile::at(32, 0) + (F / NB) * 2 * Tile::kChunkStride>(ka);
         };
+        matrix_phase(true);
         unrolled<0, kAhead>(ask);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -478,79 +522,75 @@ shaped_kernel(const ShapedParams p) {
           acc[F % NB] = mma_chunk<T>(kf[F], qf[F / NB], acc[F % NB]);
           if constexpr (F + kAhead < kFrags) ask(std::integral_constant<int, F + kAhead>{});
         });
+        matrix_phase(false);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[nb][r] = acc[nb][r];
       }
 
+      // ---- z, relative to the running maximum: one multiply-add away from the products (or from the tanh), so that
+      // 2^z needs no subtraction. A cache key's bias is linear in the constant part of its index.
       const bool whole_tile = !tree && key0 >= wave_lo && key0 + kKeys <= T_b;   // seen by every row of the wave
-      const bool raw = whole_tile && growing;   // the maximum is taken from the raw products
-      if (!raw) {
-        if (capped) {
+      const float m_use = m_run == neg_inf() ? 0.f : m_run;
+      const float away = static_cast<float>(pos - lane_key);
+      const float base = (capped && !kIs32<T> ? cap2 : 0.f) - m_use - (tree ? 0.f : slope * away);
+      auto shape = [&](auto capped_c, auto sloped_c) __attribute__((always_inline)) {
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[nb][r] = __builtin_fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(ex * s[nb][r])), cap2);
-        } else {
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[nb][r] *= c;
-        }
-        if (tree) {
-          tree_scores(s, key0, lane_key);
-        } else {
-          if (p.slopes) {
-            const float away = static_cast<float>(pos - lane_key);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[nb][r] = __builtin_fmaf(-slope, away - static_cast<float>(key_of(nb, r)), s[nb][r]);
+          for (int r = 0; r < 16; ++r) {
+            pin(s[nb][r]);
+            float z;
+            if constexpr (!decltype(capped_c)::value) z = __builtin_fmaf(c, s[nb][r], base);
+            else if constexpr (kIs32<T>) z = __builtin_fmaf(cap2, tanhf(ex * s[nb][r]), base);   // (the form below is 2^-23 cap off, which f32 results show)
+            else z = __builtin_fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(ex * s[nb][r])), base);
+            if constexpr (decltype(sloped_c)::value) z = __builtin_fmaf(slope, static_cast<float>(key_of(nb, r)), z);
+            s[nb][r] = z;
           }
-          if (!whole_tile) {
-            const int from_key = row_lo - lane_key, keys_left = T_b - lane_key;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[nb][r] = key_of(nb, r) >= from_key && key_of(nb, r) < keys_left ? s[nb][r] : neg_inf();
-          }
-        }
+      };
+      if (capped) {
+        if (sloped && !tree) shape(std::true_type{}, std::true_type{}); else shape(std::true_type{}, std::false_type{});
+      } else {
+        if (sloped && !tree) shape(std::false_type{}, std::true_type{}); else shape(std::false_type{}, std::false_type{});
       }
-      if (tree) clear_unseen(s, smem + kVRing + stage);
-      if (!wave_active) continue;
+      if (tree) {
+        tree_scores(s, key0, lane_key);
+        clear_unseen(s, smem + kVRing + stage);
+        if (!wave_active) continue;
+      } else if (!whole_tile) {
+        const int from_key = row_lo - lane_key, keys_left = T_b - lane_key;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[nb][r] = key_of(nb, r) >= from_key && key_of(nb, r) < keys_left ? s[nb][r] : neg_inf();
+      }
       float top = s[0][0];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
-      if (raw) top = capped ? __builtin_fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(ex * top)), cap2) : c * top;
-      // The maximum only has to keep the weights in range: it moves, and O and l are rescaled, when a row's scores
-      // pass it by more than 8 (weights up to 2^8).
-      if (wave_any(top > m_run + 8.f)) {
-        const float m_new = fmaxf(m_run, half_swap_max(top, lh));
-        const float a = m_new == neg_inf() ? 1.f : fast_exp2(m_run - m_new);
+      // The maximum only has to keep the weights in range: it moves, and O and l are rescaled, when a row has no
+      // maximum yet or its scores pass it by more than 8 (weights up to 2^8).
+      if (wave_any(top > (m_run == neg_inf() ? neg_inf() : 8.f))) {
+        const float m_new = fmaxf(m_run, m_use + half_swap_max(top, lh));
+        const float shift = m_new == neg_inf() ? 0.f : m_new - m_use;
+        const float a = m_run == neg_inf() ? 1.f : fast_exp2(-shift);   // (l and O are 0 where there was no maximum)
         m_run = m_new;
         l_run *= a;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[db][r] *= a;
-      }
-      const float m_use = m_run == neg_inf() ? 0.f : m_run;
-      if (raw && capped) {
-        const float base = cap2 - m_use;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[nb][r] = fast_exp2(__builtin_fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(ex * s[nb][r])), base));
-      } else {
-        const float times = raw ? c : 1.f;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[nb][r] = fast_exp2(__builtin_fmaf(times, s[nb][r], -m_use));
+          for (int r = 0; r < 16; ++r) s[nb][r] -= shift;
       }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[nb][r] = fast_exp2(s[nb][r]);
 
       // ---- O^T += V^T P^T
       const uint32_t va = v_rd + stage;
@@ -601,6 +641,7 @@ shaped_kernel(const ShapedParams p) {
           vlo[G] = lds_read_tr16_b64<kOff>(va);
           vhi[G] = lds_read_tr16_b64<kOff + kRows8>(va);
         };
+        matrix_phase(true);
         unrolled<0, kAhead>(ask);
         unrolled<0, kFrags>([&](auto g) __attribute__((always_inline)) {
           constexpr int G = decltype(g)::value;
@@ -609,6 +650,7 @@ shaped_kernel(const ShapedParams p) {
           o[G % DB] = M::mma(__builtin_bit_cast(typename M::Vec8, raw_v), pf[G / DB], o[G % DB]);
           if constexpr (G + kAhead < kFrags) ask(std::integral_constant<int, G + kAhead>{});
         });
+        matrix_phase(false);
       }
     }
 
@@ -690,37 +732,52 @@ shaped_kernel(const ShapedParams p) {
   }
 }
 
-// Joins the partials of the pairs that were cut. One workgroup per few rows of a pair, four columns a thread.
+// Joins the partials of the pairs that were cut. One workgroup per few rows of a pair, four columns a thread; the
+// partials of up to kTogether stretches are in flight together (they come from other XCDs' workgroups, so every
+// one is a round trip to memory).
 template <typename T, int D, int WK>
 __global__ void __launch_bounds__(256) shaped_join_kernel(const ShapedParams p) {
-  constexpr int kKeys = kTileKeys<T>, kRowsPerWg = 128 / WK, kRowsPerBlock = 256 / (D / 4);
+  constexpr int kKeys = kTileKeys<T>, kRowsPerWg = 128 / WK, kRowsPerBlock = 256 / (D / 4), kTogether = 8;
   const int per_pair = (p.rows + kRowsPerBlock - 1) / kRowsPerBlock;
   const int pair = blockIdx.x / per_pair;
-  const int b = pair / p.units, unit = pair % p.units;
+  const int unit = pair % p.units;
   const int row = (blockIdx.x % per_pair) * kRowsPerBlock + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-  int before, total;
-  line_sums<kKeys>(p, b, &before, &total);
-  const int stretch = stretch_of(p, total);
-  const int n = sequence_of<kKeys>(p, b).n;
-  const int begin = before * p.units + unit * n;
-  const int g0 = begin / stretch, g1 = (begin + n - 1) / stretch;
+  const Place here = place_of<kKeys>(p, true, [&](int) { return pair / p.units; });
+  const Stretches cut = cut_line(p, here.total);
+  const int begin = here.begin + unit * here.seq.n;
+  const int g0 = cut.holder(begin), g1 = cut.holder(begin + here.seq.n - 1);
   if (g0 == g1 || row >= p.rows) return;
   const int row_block = row / kRowsPerWg, local = row % kRowsPerWg;
-  auto part = [&](int g) {
-    return p.partial + ((static_cast<int64_t>(row_block) * p.groups + g) * 2 + (begin < g * stretch ? 0 : 1)) * p.partial_floats;
-  };
-  float m = neg_inf();
-  for (int g = g0; g <= g1; ++g) m = fmaxf(m, part(g)[p.rows_cap * D + 2 * local]);
+  const int64_t stats = static_cast<int64_t>(p.rows_cap) * D + 2 * local, values = static_cast<int64_t>(local) * D + d;
+  float m = neg_inf(), l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  if (m != neg_inf()) {
-    for (int g = g0; g <= g1; ++g) {
-      const float* at = part(g);
-      const float w = fast_exp2(at[p.rows_cap * D + 2 * local] - m);
-      const f32x4 o = *reinterpret_cast<const f32x4*>(at + static_cast<int64_t>(local) * D + d);
-      l += w * at[p.rows_cap * D + 2 * local + 1];
+  for (int g = g0; g <= g1; g += kTogether) {
+    f32x2 ml[kTogether];
+    f32x4 o[kTogether];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += w * o[e];
+    for (int i = 0; i < kTogether; ++i) {
+      if (g + i > g1) continue;
+      const float* part = p.partial + ((static_cast<int64_t>(row_block) * p.groups + g + i) * 2 + (begin < cut.start(g + i) ? 0 : 1)) * p.partial_floats;
+      ml[i] = *reinterpret_cast<const f32x2*>(part + stats);
+      o[i] = *reinterpret_cast<const f32x4*>(part + values);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i)
+      if (g + i <= g1) top = fmaxf(top, ml[i][0]);
+    if (top == neg_inf()) continue;
+    const float keep = fast_exp2(m - top);
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      if (g + i > g1) continue;
+      const float w = fast_exp2(ml[i][0] - top);
+      l += w * ml[i][1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += w * o[i][e];
     }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -729,26 +786,27 @@ __global__ void __launch_bounds__(256) shaped_join_kernel(const ShapedParams p) 
   Vec4 v4;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(acc[e] * inv);
-  *reinterpret_cast<Vec4*>(static_cast<T*>(p.out) + b * p.out_stride[0] + head * p.out_stride[1] + i * p.out_stride[2] + d) = v4;
+  *reinterpret_cast<Vec4*>(static_cast<T*>(p.out) + here.b * p.out_stride[0] + head * p.out_stride[1] + i * p.out_stride[2] + d) = v4;
 }
 
 // ---------------------------------------------------------------------------------------------- host
 struct Cut {
-  int key_waves, rows_per_wg, row_blocks, heads_per_unit, units, rows, groups, whole, rows_cap, tree_tiles;
+  int key_waves, rows_per_wg, row_blocks, heads_per_unit, units, rows, groups, whole, rows_cap, tree_tiles, lead_groups, lead_permille;
   int64_t partial_floats, bytes;
 };
 
 int cut_of(const fta_shaped_args& a, int num_cus, Cut* out) {
   if (num_cus <= 0) num_cus = kDefaultCUs;
   Cut c{};
-  const int keys = a.dtype == FTA_F32 ? 32 : 64;
+  const bool is32 = a.dtype == FTA_F32;
+  const int keys = is32 ? 32 : 64;
   c.heads_per_unit = a.cur_heads == a.num_kv_heads ? a.num_q_heads / a.num_kv_heads : 1;
   c.units = a.num_q_heads / c.heads_per_unit;
   const int64_t rows = static_cast<int64_t>(c.heads_per_unit) * a.q_len;
   if (rows > 1 << 24) return FTA_ERR_SHAPE;
   c.rows = static_cast<int>(rows);
   // Units of up to 64 rows: two waves per 32 rows, so that all four compute.
-  c.key_waves = a.dtype != FTA_F32 && c.rows <= 64 ? 2 : 1;
+  c.key_waves = !is32 && c.rows <= 64 ? 2 : 1;
   c.rows_per_wg = 128 / c.key_waves;
   c.row_blocks = (c.rows + c.rows_per_wg - 1) / c.rows_per_wg;
   c.tree_tiles = (a.q_len + keys - 1) / keys;
@@ -762,6 +820,16 @@ int cut_of(const fta_shaped_args& a, int num_cus, Cut* out) {
   c.whole = cap_tiles <= 2 * kMinStretch;
   c.groups = c.whole ? static_cast<int>(pairs) : std::max(1, num_cus * per_cu / c.row_blocks);
   c.rows_cap = std::min(c.rows, c.rows_per_wg);
+  // Where a CU holds two workgroups, the one that came first has the older waves, which the scheduler serves first:
+  // with a cap and a bias it takes 2.7 us a tile, the other one 3.3, and equal stretches leave the CU half empty at
+  // the end. The first half of the stretches gets 57 % of the line: 64 sequences up to 32768 keys, 64 heads on 8,
+  // 16 nodes 820 us against 851, 8 x 32768, 32 on 8, 64 nodes 371 against 395, head_dim 64 169 against 176. With a
+  // cap or a bias alone it is even (268 against 265) or loses (258 against 244), and is not done.
+  c.lead_groups = c.lead_permille = 0;
+  if (!c.whole && per_cu == 2 && !is32 && c.key_waves == 1 && a.softcap > 0.f && a.slopes && c.groups >= 2) {
+    c.lead_groups = c.groups / 2;
+    c.lead_permille = 570;
+  }
   c.partial_floats = (static_cast<int64_t>(c.rows_cap) * (a.head_dim + 2) + 3) / 4 * 4;
   c.bytes = c.whole ? 0 : static_cast<int64_t>(c.row_blocks) * c.groups * 2 * c.partial_floats * 4;
   *out = c;
@@ -885,6 +953,7 @@ int fta_shaped_decode(const fta_shaped_args* args, void* hip_stream) {
   p.heads_per_unit = c.heads_per_unit; p.units = c.units;
   p.kv_group = a.num_q_heads / a.num_kv_heads; p.cur_group = a.num_q_heads / a.cur_heads;
   p.rows = c.rows; p.row_blocks = c.row_blocks; p.groups = c.groups; p.tree_tiles = c.tree_tiles; p.whole = c.whole; p.rows_cap = c.rows_cap;
+  p.lead_groups = c.lead_groups; p.lead_permille = c.lead_permille;
   p.len_is_i64 = a.len_dtype == FTA_I64; p.mask_packed = a.mask_kind == FTA_MASK_PACKED_U64;
   p.page_shift = a.page_size == 16 ? 4 : a.page_size == 32 ? 5 : a.page_size == 64 ? 6 : 7;
   p.window = a.window; p.scale = a.sm_scale; p.softcap = a.softcap;

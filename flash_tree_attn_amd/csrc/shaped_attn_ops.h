@@ -37,6 +37,15 @@ __device__ __forceinline__ const __attribute__((address_space(4))) P* parameters
   return at;
 }
 
+// Pins a value to this place: arithmetic on it stays behind, where the compiler would otherwise do the cheap first
+// operation of one branch ahead of the branch, for the other one in vain.
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
+
+// A wave in its matrix products goes ahead of one in its vector arithmetic, which then runs between the products.
+__device__ __forceinline__ void matrix_phase(bool on) {
+  if (on) __builtin_amdgcn_s_setprio(1); else __builtin_amdgcn_s_setprio(0);
+}
+
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
 }  // namespace
