@@ -301,7 +301,7 @@ shaped_kernel(const ShapedParams p) {
     const int32_t* table = PAGED ? p.table + b * p.table_stride : nullptr;
 
     // pages of the blocks of the next cache tile, requested when the one ahead of it goes out
-    int page_of[kLoads];
+    int page_of[kLoads], at0 = 0;
     auto look_up = [&](int tile) __attribute__((always_inline)) {
       if constexpr (PAGED) {
 #pragma unroll
@@ -337,34 +337,46 @@ shaped_kernel(const ShapedParams p) {
       request_rows(std::true_type{}, t, (u0 + t) * kKeys, static_cast<const char*>(c->ck) + (b * c->ck_stride[0] + cur_head * c->ck_stride[1]) * ES,
                    static_cast<const char*>(c->cv) + (b * c->cv_stride[0] + cur_head * c->cv_stride[1]) * ES, c->ck_stride[2] * ES, c->cv_stride[2] * ES, 0, L - 1);
     };
+    // Where tile t's blocks come from and go to, if it is a cache tile that lies in [lo, T) as a whole.
+    const char* ksrc;
+    const char* vsrc;
+    char* kst;
+    auto blocks_of = [&](int t) __attribute__((always_inline)) {
+      const int key0 = (last_tile - (t - trees)) * kKeys;
+      const bool whole = t >= trees && t < tiles && key0 >= seq.lo && key0 + kKeys <= T_b;
+      kst = smem + (t % kStages) * Tile::kBytes + wave * Tile::kBlockPitch;
+      ksrc = kbase + k_lane;
+      vsrc = vbase + v_lane;
+      if constexpr (PAGED) {
+        at0 = key0 + wave * RPB;
+      } else if (whole) {
+        ksrc += key0 * k_row;
+        vsrc += key0 * v_row;
+      }
+      return whole;
+    };
+    // Load q of 2 * kLoads of them: K and V of this wave's blocks in turn.
+    auto load_block = [&](auto q_c) __attribute__((always_inline)) {
+      constexpr int Q = decltype(q_c)::value, i = Q / 2;
+      constexpr bool is_v = Q % 2 != 0;
+      const char* src = is_v ? vsrc : ksrc;
+      if constexpr (PAGED) {
+        const int at = (at0 + i * 4 * RPB) & page_mask;
+        src += is_v ? page_of[i] * v_page + at * v_row : page_of[i] * k_page + at * k_row;
+      } else {
+        src += i * (is_v ? v_step : k_step);
+      }
+      FTA_LOAD_BLOCK_TO_LDS(src, kst + (is_v ? kVRing : 0) + i * 4 * Tile::kBlockPitch);
+    };
+    // Tile t in one go: the first of a pair, edges, tree tiles, and where the wave has no products to spread the loads over.
     auto request = [&](int t) __attribute__((always_inline)) {
       if (t < trees) {
         request_tree(t);
         return;
       }
-      const int tile = last_tile - (t - trees), key0 = tile * kKeys;
-      if (key0 >= seq.lo && key0 + kKeys <= T_b) {
-        char* kst = smem + (t % kStages) * Tile::kBytes;
-        char* vst = kst + kVRing;
-        if constexpr (PAGED) {
-#pragma unroll
-          for (int i = 0; i < kLoads; ++i) {
-            const int blk = i * 4 + wave, at = (key0 + blk * RPB) & page_mask;
-            FTA_LOAD_BLOCK_TO_LDS(kbase + (page_of[i] * k_page + at * k_row) + k_lane, kst + blk * Tile::kBlockPitch);
-            FTA_LOAD_BLOCK_TO_LDS(vbase + (page_of[i] * v_page + at * v_row) + v_lane, vst + blk * Tile::kBlockPitch);
-          }
-        } else {
-          const char* ksrc = kbase + key0 * k_row + k_lane;
-          const char* vsrc = vbase + key0 * v_row + v_lane;
-#pragma unroll
-          for (int i = 0; i < kLoads; ++i) {
-            FTA_LOAD_BLOCK_TO_LDS(ksrc + i * k_step, kst + (i * 4 + wave) * Tile::kBlockPitch);
-            FTA_LOAD_BLOCK_TO_LDS(vsrc + i * v_step, vst + (i * 4 + wave) * Tile::kBlockPitch);
-          }
-        }
-      } else {
-        request_rows(std::false_type{}, t, key0, kbase, vbase, k_row, v_row, seq.lo, T_b - 1);
-      }
+      const int tile = last_tile - (t - trees);
+      if (blocks_of(t)) unrolled<0, 2 * kLoads>(load_block);
+      else request_rows(std::false_type{}, t, tile * kKeys, kbase, vbase, k_row, v_row, seq.lo, T_b - 1);
       look_up(tile - 1);
     };
     if (cache_tiles > 0) look_up(last_tile);
@@ -486,18 +498,22 @@ shaped_kernel(const ShapedParams p) {
     for (int t = 0; t < tiles; ++t) {
       wait_vmcnt<0>();          // this wave's part of tile t has landed ...
       workgroup_barrier();      // ... and everybody's, and everybody is done with tile t - 1, whose stage tile t + 1 takes
-      if (t + 1 < tiles) request(t + 1);
       const bool tree = t < trees;
-      if (!wave_active && !tree) continue;
       const uint32_t stage = (t % kStages) * Tile::kBytes;
       const int key0 = (tree ? u0 + t : last_tile - (t - trees)) * kKeys;
       const int lane_key = key0 + lane_key0;
+      bool idle = !wave_active && !tree;
       // A tile whose capped scores, lowered by their distance, are all more than 2^150 below the row's maximum has
       // weights of exactly 0 in 32 bits: nothing of it would be added.
       if (capped && sloped && !tree) {
         const float nearest = static_cast<float>(pos - key0 - (kKeys - 1)), farthest = static_cast<float>(pos - key0);
-        if (!wave_any(row_ok && !(cap2 - fminf(slope * nearest, slope * farthest) < m_run + kNoWeight))) continue;
+        idle = idle || !wave_any(row_ok && !(cap2 - fminf(slope * nearest, slope * farthest) < m_run + kNoWeight));
       }
+      // The next tile's loads go out between the products: in one go they hold the wave for 900 to 1500 cycles a tile
+      // (the CU takes a wave-wide load every 16), a third of its time; spread, they cost their issue.
+      const bool spread = !idle && blocks_of(t + 1);
+      if (!spread && t + 1 < tiles) request(t + 1);
+      if (idle) continue;
 
       // ---- S^T = K Q^T, fragments requested a few products ahead
       float s[NB][16];
@@ -521,7 +537,13 @@ shaped_kernel(const ShapedParams p) {
           wait_lgkm<(kFrags - 1 - F < kAhead - 1 ? kFrags - 1 - F : kAhead - 1)>(kf[F]);
           acc[F % NB] = mma_chunk<T>(kf[F], qf[F / NB], acc[F % NB]);
           if constexpr (F + kAhead < kFrags) ask(std::integral_constant<int, F + kAhead>{});
+          constexpr int kFrom = F * 2 * kLoads / kFrags, kTo = (F + 1) * 2 * kLoads / kFrags;
+          if constexpr (kTo > kFrom) {
+            if (spread) unrolled<kFrom, kTo>(load_block);
+            schedule_fence();
+          }
         });
+        if (spread) look_up(last_tile - (t + 1 - trees) - 1);
         matrix_phase(false);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
