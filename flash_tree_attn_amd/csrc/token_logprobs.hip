@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "fta_device.h"
 
@@ -81,10 +82,19 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t x) {
   return x;
 }
 
-// Results of one row, by all threads of the block: statistics (m, l, t), and the k largest entries in `top`
-// (LDS, descending; 0 where the row has none left).
+// The logit of the row's token j: requested at the start of a kernel, so that the two round trips (the id, then its
+// logit) pass under everything else. -inf outside the vocabulary.
 template <typename T>
-__device__ __forceinline__ void write_row(const LogprobParams& p, int64_t row, float m, float l, float t, const uint64_t* top) {
+__device__ __forceinline__ float logit_of_id(const LogprobParams& p, int64_t row, int j) {
+  const int64_t at = row * p.id_stride[0] + j * p.id_stride[1];
+  const int64_t id = p.id_is_i64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<int64_t>(static_cast<const int32_t*>(p.ids)[at]);
+  return id >= 0 && id < p.vocab ? to_f32(static_cast<const T*>(p.logits)[row * p.logits_stride + id]) : neg_inf();
+}
+
+// Results of one row, by all threads of the block: statistics (m, l, t), the logit of token threadIdx.x, and the k
+// largest entries in `top` (LDS, descending; 0 where the row has none left).
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobParams& p, int64_t row, float m, float l, float t, float token_logit, const uint64_t* top) {
   const bool empty = l == 0.f;                      // every logit is -inf
   const float log_l = empty ? 0.f : logf(l);
   auto logprob = [&](float x) { return empty ? neg_inf() : (x - m) * p.inv_temp - log_l; };
@@ -92,12 +102,8 @@ __device__ __forceinline__ void write_row(const LogprobParams& p, int64_t row, f
     p.lse[row] = empty ? neg_inf() : m * p.inv_temp + log_l;
     p.entropy[row] = empty ? 0.f : log_l - kLn2 * (t / l);
   }
-  const T* x = static_cast<const T*>(p.logits) + row * p.logits_stride;
-  for (int j = threadIdx.x; j < p.num_ids; j += blockDim.x) {
-    const int64_t at = row * p.id_stride[0] + j * p.id_stride[1];
-    const int64_t id = p.id_is_i64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<int64_t>(static_cast<const int32_t*>(p.ids)[at]);
-    p.logprobs[row * p.num_ids + j] = id >= 0 && id < p.vocab ? logprob(to_f32(x[id])) : neg_inf();
-  }
+  for (int j = threadIdx.x; j < p.num_ids; j += blockDim.x)
+    p.logprobs[row * p.num_ids + j] = logprob(j < static_cast<int>(blockDim.x) ? token_logit : logit_of_id<T>(p, row, j));
   for (int j = threadIdx.x; j < p.top_k; j += blockDim.x) {
     p.top_logprobs[row * p.top_k + j] = logprob(value_of(static_cast<uint32_t>(top[j] >> 32)));
     p.top_ids[row * p.top_k + j] = index_of(top[j]);
@@ -158,14 +164,16 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
     }
   }
   const float stray = stray_at >= 0 ? to_f32(x[stray_at]) : neg_inf();
+  const float token_logit = p.chunks == 1 && tid < p.num_ids ? logit_of_id<T>(p, row, tid) : neg_inf();
 
-  float mine = stray;
+  float mine = stray, mine_number = stray;   // the largest, NaN if there is one; the largest number
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
     const Granule g = __builtin_bit_cast(Granule, raw[j]);
 #pragma unroll
     for (int e = 0; e < kVec; ++e) mine = max_or_nan(mine, to_f32(g.v[e]));
   }
+  if (mine != mine) mine_number = __builtin_huge_valf(); else mine_number = mine;   // (with a NaN: look at all of them)
   float m = mine;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = max_or_nan(m, __shfl_xor(m, o, 64));
@@ -179,28 +187,35 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
 
   // wave 0 searches the threshold while the others sum
   if (p.top_k > 0 && wave == 0) {
-    const int per = p.top_k <= 32 ? 1 : 4;   // groups per lane: k of 64 groups' maxima, k up to 128 of 256
+    // the maxima of 64 groups of threads for k up to 32, of 256 for k up to 128
     uint32_t key[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const uint32_t u = s_key[w * 64 + lane];
-      if (per == 1) key[0] = max(key[0], u); else key[w % 4] = max(key[w % 4], u);
-    }
-    uint32_t threshold = 0;
-    for (int bit = 31; bit >= 12; --bit) {   // the low bits stay zero: a slightly lower threshold, a few more candidates
-      const uint32_t trial = threshold | 1u << bit;
-      int reach = 0;
+    for (int w = 0; w < kWaves; ++w) key[w % 4] = max(key[w % 4], s_key[w * 64 + lane]);
+    auto search = [&](auto groups_c) __attribute__((always_inline)) {
+      uint32_t found = 0;
+      for (int bit = 31; bit >= 12; --bit) {   // the low bits stay zero: a slightly lower threshold, a few more candidates
+        const uint32_t trial = found | 1u << bit;
+        int reach = 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] >= trial));
-      if (reach >= p.top_k) threshold = trial;
+        for (int r = 0; r < decltype(groups_c)::value; ++r) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] >= trial));
+        if (reach >= p.top_k) found = trial;
+      }
+      return found;
+    };
+    uint32_t threshold;
+    if (p.top_k <= 32) {
+      key[0] = max(max(key[0], key[1]), max(key[2], key[3]));
+      threshold = search(std::integral_constant<int, 1>{});
+    } else {
+      threshold = search(std::integral_constant<int, 4>{});
     }
     if (lane == 0) s_threshold = threshold;
   }
 
-  const float scale = p.inv_temp * kLog2e, m_use = m == neg_inf() ? 0.f : m;
+  const float scale = p.inv_temp * kLog2e, m_scaled = m == neg_inf() ? 0.f : m * scale;
   float l = 0.f, t = 0.f;
   auto add = [&](float v) __attribute__((always_inline)) {
-    const float d = max_or_nan((v - m_use) * scale, -256.f);   // 2^-256 is 0 in 32 bits; keeps 0 * inf out of t
+    const float d = max_or_nan(__builtin_fmaf(v, scale, -m_scaled), -256.f);   // 2^-256 is 0 in 32 bits; keeps 0 * inf out of t
     const float w = fast_exp2(d);
     l += w;
     t = __builtin_fmaf(w, d, t);
@@ -227,12 +242,20 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
     l += s_l[w];
     t += s_t[w];
   }
+  {
+    // the exponents were taken against m scale rounded: off by the same `off` in every one
+    const float off = m == neg_inf() ? 0.f : __builtin_fmaf(m, scale, -m_scaled), back = exp2f(-off);
+    t = back * __builtin_fmaf(-off, l, t);
+    l *= back;
+  }
 
   if (p.top_k > 0) {
-    const uint32_t threshold = max(s_threshold, 1u);
-    if (s_key[tid] >= threshold) {
+    // Where the threshold is not a number's (fewer than k logits that are) the k largest are extracted one by one.
+    const bool few = s_threshold < key_of(neg_inf());
+    const float least = value_of(max(s_threshold, key_of(neg_inf())));
+    if (!few && mine_number >= least) {
       auto collect = [&](float v, int at) __attribute__((always_inline)) {
-        if (key_of(v) < threshold) return;
+        if (!(v >= least)) return;
         const int slot = atomicAdd(&s_count, 1);
         if (slot < kSlots) s_entry[slot] = entry_of(v, at);
       };
@@ -242,14 +265,17 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
         FTA_FORGET(raw[j]);
         const Granule g = __builtin_bit_cast(Granule, raw[j]);
         const int e0 = first + j * NT * kVec;
-        if (e0 < 0 || e0 + kVec > p.vocab) continue;
+        float best = to_f32(g.v[0]);
+#pragma unroll
+        for (int e = 1; e < kVec; ++e) best = fmaxf(best, to_f32(g.v[e]));
+        if (!(best >= least) || e0 < 0 || e0 + kVec > p.vocab) continue;   // most granules, for all lanes of a wave
 #pragma unroll
         for (int e = 0; e < kVec; ++e) collect(to_f32(g.v[e]), e0 + e);
       }
     }
     __syncthreads();
     const int n = s_count;
-    if (n <= kSlots) {
+    if (n <= kSlots && !few) {
       rank_entries(s_entry, n, p.top_k, s_top);
     } else {
       uint64_t last = ~0ull;
@@ -278,13 +304,17 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
         if (tid == 0) s_top[k] = best;
         last = best;
         __syncthreads();   // s_best is free again
+        if (best == 0) {   // none left
+          for (int i = k + tid; i < p.top_k; i += NT) s_top[i] = 0;
+          break;
+        }
       }
     }
     __syncthreads();
   }
 
   if (p.chunks == 1) {
-    write_row<T>(p, row, m, l, t, s_top);
+    write_row<T>(p, row, m, l, t, token_logit, s_top);
     return;
   }
   char* out = p.workspace + (row * p.chunks + chunk) * chunk_bytes(p.top_k);
@@ -301,19 +331,32 @@ __global__ void __launch_bounds__(256) logprob_join_kernel(const LogprobParams p
   __shared__ uint64_t s_top[kMaxTop];
   const int64_t row = blockIdx.x;
   const char* ws = p.workspace + row * p.chunks * chunk_bytes(p.top_k);
-  auto stats = [&](int c) { return *reinterpret_cast<const ChunkStats*>(ws + c * chunk_bytes(p.top_k)); };
-  // every thread joins all chunks: few, and the same addresses in every lane
-  float m = neg_inf();
-  for (int c = 0; c < p.chunks; ++c) m = max_or_nan(m, stats(c).m);
+  const float token_logit = static_cast<int>(threadIdx.x) < p.num_ids ? logit_of_id<T>(p, row, threadIdx.x) : neg_inf();
+  // every wave joins the chunks, one per lane
+  const int lane = threadIdx.x & 63;
   const float scale = p.inv_temp * kLog2e;
-  float l = 0.f, t = 0.f;
-  for (int c = 0; c < p.chunks; ++c) {
-    const ChunkStats s = stats(c);
-    if (s.m == neg_inf()) continue;
-    const float shift = (s.m - m) * scale;            // NaN where m is NaN or +inf, and so are l and t then
-    const float w = exp2f(shift);
-    l += w * s.l;
-    if (w != 0.f) t += w * (s.t + shift * s.l);   // (a NaN weight is not 0)
+  float m = neg_inf(), l = 0.f, t = 0.f;
+  for (int c0 = 0; c0 < p.chunks; c0 += 64) {
+    ChunkStats s{neg_inf(), 0.f, 0.f, 0.f};
+    if (c0 + lane < p.chunks) s = *reinterpret_cast<const ChunkStats*>(ws + (c0 + lane) * chunk_bytes(p.top_k));
+    float top = s.m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor(top, o, 64));
+    top = max_or_nan(top, m);
+    auto moved = [&](float from, float sum, float weighted, float* to_sum, float* to_weighted) {
+      *to_sum = *to_weighted = 0.f;
+      if (from == neg_inf()) return;
+      const float shift = (from - top) * scale;          // NaN where the maximum is NaN or +inf, and so are l and t then
+      const float w = exp2f(shift);
+      *to_sum = w * sum;
+      if (w != 0.f) *to_weighted = w * (weighted + shift * sum);   // (a NaN weight is not 0)
+    };
+    float sum, weighted, sum_before, weighted_before;
+    moved(s.m, s.l, s.t, &sum, &weighted);
+    moved(m, l, t, &sum_before, &weighted_before);
+    l = wave_sum(sum) + sum_before;
+    t = wave_sum(weighted) + weighted_before;
+    m = top;
   }
   if (p.top_k > 0) {
     // as many chunks' keys at a time as fit next to the best so far
@@ -342,7 +385,7 @@ __global__ void __launch_bounds__(256) logprob_join_kernel(const LogprobParams p
       }
     }
   }
-  write_row<T>(p, row, m, l, t, s_top);
+  write_row<T>(p, row, m, l, t, token_logit, s_top);
 }
 
 // How a call is cut. A row that one workgroup of 1024 threads holds in registers takes one launch and is the
@@ -352,9 +395,10 @@ struct Cut {
   bool whole_rows;
   int chunks;
 };
-Cut cut_of(const fta_logprob_args& a) {
+// `aligned`: every row starts 16-byte aligned, which is only known with the pointer; the workspace is sized without.
+Cut cut_of(const fta_logprob_args& a, bool aligned) {
   const int vec = a.dtype == FTA_F32 ? 4 : 8;
-  const int64_t span = static_cast<int64_t>(a.vocab) + vec - 1;   // with the largest possible lead
+  const int64_t span = static_cast<int64_t>(a.vocab) + (aligned ? 0 : vec - 1);   // with the largest possible lead
   Cut c;
   c.whole_rows = a.rows <= 128 && span <= 1024 * 16 * vec;
   c.chunks = c.whole_rows ? 1 : static_cast<int>((span + 512 * 8 * vec - 1) / (512 * 8 * vec));
@@ -371,7 +415,7 @@ int validate_sizes(const fta_logprob_args& a) {
 }
 
 int64_t workspace_bytes(const fta_logprob_args& a) {
-  const Cut c = cut_of(a);
+  const Cut c = cut_of(a, false);
   return c.chunks == 1 ? 0 : a.rows * c.chunks * chunk_bytes(a.top_k);
 }
 
@@ -414,7 +458,8 @@ int fta_logprobs(const fta_logprob_args* args, void* hip_stream) {
     if (a.workspace_bytes < need) return FTA_ERR_SCRATCH_TOO_SMALL;
     if (reinterpret_cast<uintptr_t>(a.workspace) % 16) return FTA_ERR_STRIDE;
   }
-  const Cut cut = cut_of(a);
+  const int es = a.dtype == FTA_F32 ? 4 : 2;
+  const Cut cut = cut_of(a, reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && (a.rows == 1 || a.logits_stride * es % 16 == 0));
   LogprobParams p{};
   p.logits = a.logits; p.ids = a.token_ids; p.logprobs = a.logprobs; p.entropy = a.entropy; p.lse = a.lse;
   p.top_logprobs = a.top_logprobs; p.top_ids = a.top_ids; p.workspace = static_cast<char*>(a.workspace);
