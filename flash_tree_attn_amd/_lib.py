@@ -130,6 +130,7 @@ class FtaError(RuntimeError):
 
 
 _lib = None
+_binding = None
 
 
 def load() -> C.CDLL:
@@ -183,3 +184,16 @@ def check(status: int) -> None:
         err.status = status
         raise err
     raise FtaError(status, text)
+
+
+def binding():
+    """The native module of repeat calls (csrc/binding.cpp); raises, never falls back, when it has not been built."""
+    global _binding
+    if _binding is None:
+        try:
+            from . import _binding as module
+        except ImportError as error:
+            raise ImportError("flash_tree_attn_amd/_binding.so is missing or does not fit this torch: build it with "
+                              "`python -m flash_tree_attn_amd.build`") from error
+        _binding = module
+    return _binding

@@ -8,12 +8,14 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB_PATH = os.path.join(HERE, "libfta.so")
+BINDING_PATH = os.path.join(HERE, "_binding.so")
 SOURCES = ["fta_host.cpp", "stage1_shuffle.hip", "stage1_mfma.hip", "stage1_mfma_wide.hip", "stage1_mfma_splitkeys.hip", "stage2_merge.hip", "append_kv.hip",
            "rotary.hip", "token_logprobs.hip", "accept_path.hip", "shaped_attn.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -52,6 +54,20 @@ def _link(objs, path: str) -> None:
         raise RuntimeError(f"link failed:\n{res.stderr}")
 
 
+def _build_binding(path: str) -> None:
+    """The interpreter's side of repeat calls (host code only, against the torch that will load it)."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    includes = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in includes), os.path.join(CSRC, "binding.cpp"),
+           f"-L{root}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", f"-Wl,-rpath,{root}/lib", "-o", path]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building the binding failed:\n{res.stderr}")
+
+
 def _generate() -> None:
     """Rewrites csrc/wide_loop_asm.inc from its generator (deterministic; the file is committed)."""
     import importlib.util
@@ -66,13 +82,15 @@ def _generate() -> None:
 
 
 def build(verbose: bool = True) -> str:
-    """Compiles every HIP source of the library and links it."""
+    """Compiles every HIP source of the library and links it, and the binding of repeat calls."""
     _generate()
     with ThreadPoolExecutor(max_workers=min(6, len(SOURCES))) as pool:
+        binding = pool.submit(_build_binding, BINDING_PATH)
         objs = list(pool.map(_compile, SOURCES))
+        binding.result()
     _link(objs, LIB_PATH)
     if verbose:
-        print(f"built {LIB_PATH}")
+        print(f"built {LIB_PATH} and {BINDING_PATH}")
     return LIB_PATH
 
 

@@ -338,24 +338,30 @@ def _sig(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
-def _remembered(key, on: torch.Tensor):
-    """(args, byref(args), device index) that `_remember_call` kept under `key`, or None where the call has to be
-    checked in full (nothing kept, or the tensors live on another device than the current one)."""
-    entry = _fast.__dict__.get("entries", {}).get(key)
-    return entry if entry is not None and torch.cuda.current_device() == entry[2] else None
+def _calls() -> dict:
+    """This thread's remembered calls (csrc/binding.cpp)."""
+    try:
+        return _fast.calls
+    except AttributeError:
+        _fast.calls = {}
+        return _fast.calls
 
 
-def _remember_call(key, args, device, originals, used) -> None:
-    """Keeps the filled arguments of a call signature if the kernel read the caller's tensors as they came."""
-    if key is None or device.index is None:
+def _remember_call(signature, function, args, device, inputs, outputs) -> None:
+    """Keeps a checked call under the signature that `recall` formed, if the kernel read the caller's tensors as they
+    came. inputs: (field, argument, the caller's tensor, the one read), outputs: (field, argument or -1, tensor);
+    `argument` counts behind the cache, and outputs without one are allocated by every call."""
+    if signature is None or device.index is None:
         return
-    for o, u in zip(originals, used):
-        if o is not None and (u.data_ptr() != o.data_ptr() or u.dtype != o.dtype):
+    for _, _, given, read in inputs:
+        if given is not None and (read.data_ptr() != given.data_ptr() or read.dtype != given.dtype):
             return
-    cache = _fast.__dict__.setdefault("entries", {})
-    if len(cache) >= _FAST_MAX_ENTRIES:
-        cache.clear()
-    cache[key] = (args, C.byref(args), device.index)
+    place = lambda field: getattr(type(args), field).offset
+    has_workspace = hasattr(args, "workspace_bytes")
+    _lib.binding().remember(_calls(), signature, C.cast(function, C.c_void_p).value, bytes(args),
+                            tuple((argument, place(field)) for field, argument, given, _ in inputs if given is not None),
+                            tuple((place(field), argument, tensor) for field, argument, tensor in outputs),
+                            place("workspace") if has_workspace else 0, args.workspace_bytes if has_workspace else 0, device.index)
 
 
 def _fast_key(q, k_cache, v_cache, current_k, current_v, mask, kv_seq_len, block_size, max_seq_len_in_batch, output,

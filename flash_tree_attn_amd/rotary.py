@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .flash_decoding import _DTYPES, _as_rows, _check, _current_stream, _remembered, _remember_call, _rows_ok, _sig
+from .flash_decoding import _DTYPES, _as_rows, _calls, _check, _current_stream, _remember_call, _rows_ok
 
 _INT_DTYPES = {torch.int32: _lib.FTA_I32, torch.int64: _lib.FTA_I64}
 
@@ -81,31 +81,11 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     themselves, and must not overlap the inputs otherwise.
     """
     lib = _lib.load()
-    try:
-        key = ("rotary", _sig(q), _sig(k), _sig(positions), _sig(inv_freq), _sig(kv_seq_len), interleaved, attention_factor,
-               inverse, _sig(out_q), _sig(out_k))
-        args = _remembered(key, q)
-    except (AttributeError, TypeError):
-        key = args = None
-    if args is not None and not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
-        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is None else out_q
-        pq, po = q.data_ptr(), oq.data_ptr()
-        low = pq | po
-        a, ref, index = args
-        ok = pk = None
-        if k is not None:
-            ok = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is None else out_k
-            pk, a.out_k = k.data_ptr(), ok.data_ptr()
-            low |= pk | ok.data_ptr()
-        if not low & 15:
-            a.q, a.k, a.out_q = pq, pk, po
-            a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
-            if kv_seq_len is not None:
-                a.kv_seq_len = kv_seq_len.data_ptr()
-            status = lib.fta_rotary(ref, _current_stream(index))
-            if status:
-                _check(status)
-            return oq, ok
+    hit = _lib.binding().recall(_calls(), "rotary", q, k, positions, inv_freq, kv_seq_len, interleaved, attention_factor, inverse, out_q, out_k)
+    if hit.__class__ is tuple:
+        if hit[0]:
+            _check(hit[0])
+        return hit[1], hit[2] if k is not None else None
 
     if q.dim() != 4:
         raise ValueError(f"q must be [bsz, num_heads, q_len, head_dim], got {tuple(q.shape)}")
@@ -131,7 +111,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         raise ValueError("kv_seq_len must be an int32 / int64 tensor of bsz elements on q's device")
     if not math.isfinite(attention_factor):
         raise ValueError("attention_factor must be finite")
-    originals = (q, k, inv_freq, kv_seq_len)
+    given = (q, k, positions, inv_freq, kv_seq_len)
     oq = _out_rows("out_q", out_q, q)
     ok = None if k is None else _out_rows("out_k", out_k, k)
     q = _as_rows(q)
@@ -154,5 +134,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     a.pos_stride[:] = (positions.stride(0) if per_sequence else 0, positions.stride(-1))
     with torch.cuda.device(dev):
         _check(lib.fta_rotary(C.byref(a), _current_stream(dev.index)))
-    _remember_call(key, a, dev, originals, (q, k, inv_freq, kv_seq_len))
+    outputs = (("out_q", -1 if out_q is None else 9, oq),) + (() if k is None else (("out_k", -1 if out_k is None else 10, ok),))
+    read = (q, k, positions, inv_freq, kv_seq_len)
+    _remember_call(hit, lib.fta_rotary, a, dev, tuple(zip(("q", "k", "positions", "inv_freq", "kv_seq_len"), range(1, 6), given, read)), outputs)
     return oq, ok

@@ -13,8 +13,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .flash_decoding import (_DTYPES, FtaAssertionError, _as_rows, _check, _current_stream, _num_cus, _prepare_mask, _remember_call,
-                             _remembered, _rows_ok, _sig)
+from .flash_decoding import (_DTYPES, FtaAssertionError, _as_rows, _calls, _check, _current_stream, _num_cus, _prepare_mask, _remember_call,
+                             _rows_ok)
 
 
 def shaped_tree_attention(
@@ -40,36 +40,12 @@ def shaped_tree_attention(
     A row that sees nothing yields zeros. Returns [bsz, num_heads, q_len, head_dim] in q's dtype (in `output` if given).
     """
     lib = _lib.load()
-    try:
-        key = ("shaped", _sig(q), _sig(k_cache), _sig(v_cache), _sig(current_k), _sig(current_v), _sig(mask), _sig(kv_seq_len), softcap,
-               _sig(slopes), window, _sig(first_key), _sig(depths), max_seq_len_in_batch, _sig(output), sm_scale, kv_group_num, _sig(block_tables))
-        entry = _remembered(key, q)
-    except (AttributeError, TypeError):
-        key = entry = None
-    if entry is not None and not (torch.is_grad_enabled() and (q.requires_grad or current_k.requires_grad or current_v.requires_grad or
-                                                               k_cache.requires_grad or v_cache.requires_grad)):
-        a, ref, index = entry
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if output is None else output
-        pq, pk, pv, pck, pcv, po = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), current_k.data_ptr(), current_v.data_ptr(),
-                                    out.data_ptr())
-        if not (pq | pk | pv | pck | pcv | po) & 15:
-            a.q, a.k_cache, a.v_cache, a.cur_k, a.cur_v, a.out = pq, pk, pv, pck, pcv, po
-            a.mask, a.kv_seq_len = mask.data_ptr(), kv_seq_len.data_ptr()
-            if slopes is not None:
-                a.slopes = slopes.data_ptr()
-            if first_key is not None:
-                a.first_key = first_key.data_ptr()
-            if depths is not None:
-                a.depths = depths.data_ptr()
-            if block_tables is not None:
-                a.block_table = block_tables.data_ptr()
-            if a.workspace_bytes:
-                workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=q.device)
-                a.workspace = workspace.data_ptr()
-            status = lib.fta_shaped_decode(ref, _current_stream(index))
-            if status:
-                _check(status)
-            return out
+    hit = _lib.binding().recall(_calls(), "shaped", q, k_cache, v_cache, current_k, current_v, mask, kv_seq_len, slopes, first_key, depths, block_tables,
+                                output, softcap, window, max_seq_len_in_batch, sm_scale, kv_group_num)
+    if hit.__class__ is tuple:
+        if hit[0]:
+            _check(hit[0])
+        return hit[1]
 
     if q.dim() != 4:
         raise ValueError(f"q must be [bsz, num_heads, q_len, head_dim], got {tuple(q.shape)}")
@@ -123,7 +99,7 @@ def shaped_tree_attention(
         if not _rows_ok(out) or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
             raise ValueError("output needs unit inner stride, 16-byte aligned rows and a place of its own for every value")
 
-    originals = (q, k_cache, v_cache, current_k, current_v, mask, kv_seq_len, slopes, first_key, depths, block_tables)
+    given = (q, k_cache, v_cache, current_k, current_v, mask, kv_seq_len, slopes, first_key, depths, block_tables)
     q, k_cache, v_cache, current_k, current_v = (_as_rows(t) for t in (q, k_cache, v_cache, current_k, current_v))
     mask = _prepare_mask(mask, bsz, hq, L, dev)
     kv_seq_len = kv_seq_len.contiguous().view(-1)
@@ -164,6 +140,7 @@ def shaped_tree_attention(
         a.workspace = workspace.data_ptr()
     with torch.cuda.device(dev):
         _check(lib.fta_shaped_decode(C.byref(a), _current_stream(dev.index)))
-    used = (q, k_cache, v_cache, current_k, current_v, mask, kv_seq_len, slopes, first_key, depths, block_tables)
-    _remember_call(key, a, dev, originals, used)
+    read = (q, k_cache, v_cache, current_k, current_v, mask, kv_seq_len, slopes, first_key, depths, block_tables)
+    fields = ("q", "k_cache", "v_cache", "cur_k", "cur_v", "mask", "kv_seq_len", "slopes", "first_key", "depths", "block_table")
+    _remember_call(hit, lib.fta_shaped_decode, a, dev, tuple(zip(fields, range(1, 12), given, read)), (("out", -1 if output is None else 12, out),))
     return out

@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from .flash_decoding import _DTYPES, _check, _current_stream, _remember_call, _remembered, _sig
+from .flash_decoding import _DTYPES, _calls, _check, _current_stream, _remember_call
 
 _INT_DTYPES = {torch.int32: _lib.FTA_I32, torch.int64: _lib.FTA_I64}
 MAX_TOP_K = 128
@@ -47,26 +47,11 @@ def token_logprobs(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
     probabilities of -inf; a NaN or +inf makes its row's lse, entropy and log probabilities NaN.
     """
     lib = _lib.load()
-    try:
-        key = ("logprobs", _sig(logits), _sig(token_ids), top_k, temperature)
-        entry = _remembered(key, logits)
-    except (AttributeError, TypeError):
-        key = entry = None
-    if entry is not None and not (torch.is_grad_enabled() and logits.requires_grad):
-        a, ref, index = entry
-        dev = logits.device
-        out = _logprob_outputs(logits.shape[:-1], None if token_ids is None else token_ids.size(-1), top_k, dev)
-        _fill_outputs(a, out)
-        a.logits = logits.data_ptr()
-        if token_ids is not None:
-            a.token_ids = token_ids.data_ptr()
-        if a.workspace_bytes:
-            workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=dev)
-            a.workspace = workspace.data_ptr()
-        status = lib.fta_logprobs(ref, _current_stream(index))
-        if status:
-            _check(status)
-        return TokenLogprobs(*out)
+    hit = _lib.binding().recall(_calls(), "logprobs", logits, token_ids, top_k, temperature)
+    if hit.__class__ is tuple:
+        if hit[0]:
+            _check(hit[0])
+        return TokenLogprobs(*hit[1:]) if token_ids is not None else TokenLogprobs(None, *hit[1:])
 
     dev = logits.device
     if dev.type != "cuda":
@@ -106,7 +91,9 @@ def token_logprobs(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
         a.workspace = workspace.data_ptr()
     with torch.cuda.device(dev):
         _check(lib.fta_logprobs(C.byref(a), _current_stream(dev.index)))
-    _remember_call(key, a, dev, (logits, token_ids), (rows, ids))
+    fields = ("logprobs", "entropy", "lse", "top_logprobs", "top_ids")
+    _remember_call(hit, lib.fta_logprobs, a, dev, (("logits", 1, logits, rows), ("token_ids", 2, token_ids, ids)),
+                   tuple((f, -1, t) for f, t in zip(fields, out) if t is not None))
     return TokenLogprobs(*out)
 
 
@@ -127,49 +114,41 @@ def accept_tree_path(tree_tokens: torch.Tensor, parents: torch.Tensor, target_to
       next_token   [bsz] in target_tokens' dtype: the target at the path's last node
     """
     lib = _lib.load()
-    try:
-        key = ("accept", _sig(tree_tokens), _sig(parents), _sig(target_tokens), max_accept, len_dtype)
-        entry = _remembered(key, tree_tokens)
-    except (AttributeError, TypeError):
-        key = entry = None
-    if entry is not None:
-        a, ref, index = entry
-        dev = tree_tokens.device
-    else:
-        dev = tree_tokens.device
-        if dev.type != "cuda":
-            raise RuntimeError("accept_tree_path runs on the GPU only; there is no CPU fallback")
-        if tree_tokens.dim() != 2 or tree_tokens.numel() == 0 or target_tokens.shape != tree_tokens.shape:
-            raise ValueError("tree_tokens and target_tokens must be [bsz, q_len]")
-        bsz, L = tree_tokens.shape
-        if tuple(parents.shape) not in ((L,), (1, L), (bsz, L)):
-            raise ValueError("parents must be [q_len] or [bsz, q_len]")
-        for name, t in (("tree_tokens", tree_tokens), ("parents", parents), ("target_tokens", target_tokens)):
-            if t.dtype not in _INT_DTYPES or t.device != dev:
-                raise ValueError(f"{name} must be an int32 / int64 tensor on tree_tokens' device")
-        if max_accept is not None and int(max_accept) < 1:
-            raise ValueError("max_accept must be at least 1 (the root)")
-        if len_dtype not in _INT_DTYPES:
-            raise ValueError("len_dtype must be torch.int32 or torch.int64")
-        a = _lib.FtaAcceptArgs()
-        a.bsz, a.q_len, a.max_accept = bsz, L, L if max_accept is None else int(max_accept)
-        a.token_dtype, a.target_dtype = _INT_DTYPES[tree_tokens.dtype], _INT_DTYPES[target_tokens.dtype]
-        a.parent_dtype, a.len_dtype = _INT_DTYPES[parents.dtype], _INT_DTYPES[len_dtype]
-        a.token_stride[:], a.target_stride[:] = tree_tokens.stride(), target_tokens.stride()
-        per_sequence = parents.dim() == 2 and parents.size(0) > 1
-        a.parent_stride[:] = (parents.stride(0) if per_sequence else 0, parents.stride(-1))
-        ref, index = C.byref(a), dev.index
+    hit = _lib.binding().recall(_calls(), "accept", tree_tokens, parents, target_tokens, max_accept, len_dtype)
+    if hit.__class__ is tuple:
+        if hit[0]:
+            _check(hit[0])
+        return hit[1:]
+    dev = tree_tokens.device
+    if dev.type != "cuda":
+        raise RuntimeError("accept_tree_path runs on the GPU only; there is no CPU fallback")
+    if tree_tokens.dim() != 2 or tree_tokens.numel() == 0 or target_tokens.shape != tree_tokens.shape:
+        raise ValueError("tree_tokens and target_tokens must be [bsz, q_len]")
+    bsz, L = tree_tokens.shape
+    if tuple(parents.shape) not in ((L,), (1, L), (bsz, L)):
+        raise ValueError("parents must be [q_len] or [bsz, q_len]")
+    for name, t in (("tree_tokens", tree_tokens), ("parents", parents), ("target_tokens", target_tokens)):
+        if t.dtype not in _INT_DTYPES or t.device != dev:
+            raise ValueError(f"{name} must be an int32 / int64 tensor on tree_tokens' device")
+    if max_accept is not None and int(max_accept) < 1:
+        raise ValueError("max_accept must be at least 1 (the root)")
+    if len_dtype not in _INT_DTYPES:
+        raise ValueError("len_dtype must be torch.int32 or torch.int64")
+    a = _lib.FtaAcceptArgs()
+    a.bsz, a.q_len, a.max_accept = bsz, L, L if max_accept is None else int(max_accept)
+    a.token_dtype, a.target_dtype = _INT_DTYPES[tree_tokens.dtype], _INT_DTYPES[target_tokens.dtype]
+    a.parent_dtype, a.len_dtype = _INT_DTYPES[parents.dtype], _INT_DTYPES[len_dtype]
+    a.token_stride[:], a.target_stride[:] = tree_tokens.stride(), target_tokens.stride()
+    per_sequence = parents.dim() == 2 and parents.size(0) > 1
+    a.parent_stride[:] = (parents.stride(0) if per_sequence else 0, parents.stride(-1))
     idx = torch.empty((a.bsz, a.max_accept), dtype=torch.int32, device=dev)
     count = torch.empty(a.bsz, dtype=len_dtype, device=dev)
     token = torch.empty(a.bsz, dtype=target_tokens.dtype, device=dev)
     a.tree_tokens, a.parents, a.target_tokens = tree_tokens.data_ptr(), parents.data_ptr(), target_tokens.data_ptr()
     a.accept_idx, a.accept_len, a.next_token = idx.data_ptr(), count.data_ptr(), token.data_ptr()
-    if entry is not None:
-        status = lib.fta_accept_path(ref, _current_stream(index))
-        if status:
-            _check(status)
-    else:
-        with torch.cuda.device(dev):
-            _check(lib.fta_accept_path(ref, _current_stream(dev.index)))
-        _remember_call(key, a, dev, (), ())
+    with torch.cuda.device(dev):
+        _check(lib.fta_accept_path(C.byref(a), _current_stream(dev.index)))
+    _remember_call(hit, lib.fta_accept_path, a, dev, (("tree_tokens", 1, tree_tokens, tree_tokens), ("parents", 2, parents, parents),
+                                                      ("target_tokens", 3, target_tokens, target_tokens)),
+                   (("accept_idx", -1, idx), ("accept_len", -1, count), ("next_token", -1, token)))
     return idx, count, token
