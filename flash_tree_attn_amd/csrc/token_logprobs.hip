@@ -25,6 +25,7 @@ namespace fta {
 namespace {
 
 constexpr int kMaxTop = 128;
+constexpr int kThreads = 512;   // of a workgroup of the first launch
 
 // Ends what the compiler knows of a register's value: without it, it converts all logits to 32 bits once and keeps
 // the results from phase to phase, twice the registers of the 16-bit values and far more than there are.
@@ -110,27 +111,41 @@ __device__ __forceinline__ void write_row(const LogprobParams& p, int64_t row, f
   }
 }
 
+// How many of the first n entries are larger than `mine`. LDS answers after about 100 cycles, so four are read at a
+// time (more cost registers, and with them resident workgroups); `entry` holds a multiple of 4.
+__device__ __forceinline__ int larger(const uint64_t* entry, int n, uint64_t mine) {
+  int rank = 0;
+#pragma unroll 1
+  for (int j0 = 0; j0 < n; j0 += 4) {
+    uint64_t other[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) other[j] = entry[j0 + j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) rank += (j0 + j < n) & (other[j] > mine);
+  }
+  return rank;
+}
+
 // Ranks the n entries in `entry` (all different) and leaves the k largest in `top`, descending, 0 behind them.
 __device__ __forceinline__ void rank_entries(const uint64_t* entry, int n, int k, uint64_t* top) {
   for (int i = threadIdx.x; i < k; i += blockDim.x)
     if (i >= n) top[i] = 0;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const uint64_t mine = entry[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += entry[j] > mine;
+    const int rank = larger(entry, n, mine);
     if (rank < k) top[rank] = mine;
   }
 }
 
-template <typename T, int NT, int LOADS>
-__global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
+template <typename T, int LOADS>
+__global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobParams p) {
   constexpr int kVec = 16 / static_cast<int>(sizeof(T));
-  constexpr int kWaves = NT / 64;
-  constexpr int kSlots = NT;   // candidates that LDS holds
+  constexpr int kWaves = kThreads / 64;
+  constexpr int kSlots = kThreads;   // candidates that LDS holds
   struct alignas(16) Granule { T v[kVec]; };
   __shared__ float s_m[kWaves], s_l[kWaves], s_t[kWaves];
-  __shared__ uint32_t s_key[NT];
-  __shared__ uint64_t s_entry[kSlots];
+  __shared__ uint32_t s_key[kThreads];
+  alignas(16) __shared__ uint64_t s_entry[kSlots];
   __shared__ uint64_t s_top[kMaxTop];
   __shared__ uint64_t s_best[kWaves];
   __shared__ uint32_t s_threshold;
@@ -145,7 +160,7 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
   // loaded as such. The up to kVec - 1 logits in front of the first and behind the last of them are strays, one
   // per thread: of the first chunk's threads 0 .. kVec - 1, and of the last one's threads kVec .. 2 kVec - 1.
   const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
-  const int first = (chunk * NT * LOADS + tid) * kVec - lead;   // index of this thread's first granule's first logit (vocab <= 2^30)
+  const int first = (chunk * kThreads * LOADS + tid) * kVec - lead;   // index of this thread's first granule's first logit (vocab <= 2^30)
   const int head_end = min((kVec - lead) % kVec, p.vocab);      // strays: [0, head_end) and [tail, vocab)
   const int tail = max(head_end, (p.vocab + lead) / kVec * kVec - lead);
   int stray_at = -1;
@@ -156,7 +171,7 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
   bool any = stray_at >= 0;
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
-    const int e0 = first + j * NT * kVec;
+    const int e0 = first + j * kThreads * kVec;
     raw[j] = u32x4{kInf, kInf, kInf, kInf};
     if (e0 >= 0 && e0 + kVec <= p.vocab) {
       raw[j] = *reinterpret_cast<const u32x4*>(x + e0);
@@ -264,7 +279,7 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
       for (int j = 0; j < LOADS; ++j) {
         FTA_FORGET(raw[j]);
         const Granule g = __builtin_bit_cast(Granule, raw[j]);
-        const int e0 = first + j * NT * kVec;
+        const int e0 = first + j * kThreads * kVec;
         float best = to_f32(g.v[0]);
 #pragma unroll
         for (int e = 1; e < kVec; ++e) best = fmaxf(best, to_f32(g.v[e]));
@@ -289,7 +304,7 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
         // from memory again: rare, and a second unrolled walk over the registers would cost the common path its own
 #pragma unroll 1
         for (int j = 0; j < LOADS; ++j) {
-          const int e0 = first + j * NT * kVec;
+          const int e0 = first + j * kThreads * kVec;
           if (e0 < 0 || e0 + kVec > p.vocab) continue;
           const Granule g = *reinterpret_cast<const Granule*>(x + e0);
 #pragma unroll
@@ -305,7 +320,7 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
         last = best;
         __syncthreads();   // s_best is free again
         if (best == 0) {   // none left
-          for (int i = k + tid; i < p.top_k; i += NT) s_top[i] = 0;
+          for (int i = k + tid; i < p.top_k; i += kThreads) s_top[i] = 0;
           break;
         }
       }
@@ -320,15 +335,17 @@ __global__ void __launch_bounds__(NT) logprob_kernel(const LogprobParams p) {
   char* out = p.workspace + (row * p.chunks + chunk) * chunk_bytes(p.top_k);
   if (tid == 0) *reinterpret_cast<ChunkStats*>(out) = ChunkStats{m, l, t, 0.f};
   uint64_t* keys = reinterpret_cast<uint64_t*>(out + sizeof(ChunkStats));
-  for (int k = tid; k < p.top_k; k += NT) keys[k] = s_top[k];
+  for (int k = tid; k < p.top_k; k += kThreads) keys[k] = s_top[k];
 }
 
 // Joins the chunks of a row. One workgroup per row.
 template <typename T>
 __global__ void __launch_bounds__(256) logprob_join_kernel(const LogprobParams p) {
   constexpr int kSlots = 1024;
-  __shared__ uint64_t s_entry[kSlots];
+  alignas(16) __shared__ uint64_t s_entry[kSlots];
+  alignas(16) __shared__ uint64_t s_reach[kSlots];
   __shared__ uint64_t s_top[kMaxTop];
+  __shared__ int s_count;
   const int64_t row = blockIdx.x;
   const char* ws = p.workspace + row * p.chunks * chunk_bytes(p.top_k);
   const float token_logit = static_cast<int>(threadIdx.x) < p.num_ids ? logit_of_id<T>(p, row, threadIdx.x) : neg_inf();
@@ -359,24 +376,41 @@ __global__ void __launch_bounds__(256) logprob_join_kernel(const LogprobParams p
     m = top;
   }
   if (p.top_k > 0) {
-    // as many chunks' keys at a time as fit next to the best so far
+    // As many chunks' keys at a time as fit next to the best so far. Ranking them all by counting takes n^2 steps (20 us
+    // for 320 keys), so the k-th largest value is searched first, bit by bit, and what reaches it is ranked.
     const int step = (kSlots - p.top_k) / p.top_k;
     int kept = 0;
     for (int c0 = 0; c0 < p.chunks; c0 += step) {
-      const int n = min(step, p.chunks - c0) * p.top_k;
-      for (int i = threadIdx.x; i < n; i += 256)
-        s_entry[kept + i] = reinterpret_cast<const uint64_t*>(ws + (c0 + i / p.top_k) * chunk_bytes(p.top_k) + sizeof(ChunkStats))[i % p.top_k];
-      __syncthreads();
-      // missing entries (0) tie among themselves: only real ones are ranked, the rest of `top` is 0
-      for (int i = threadIdx.x; i < p.top_k; i += 256) s_top[i] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < kept + n; i += 256) {
-        const uint64_t mine = s_entry[i];
-        if (mine == 0) continue;
-        int rank = 0;
-        for (int j = 0; j < kept + n; ++j) rank += s_entry[j] > mine;
-        if (rank < p.top_k) s_top[rank] = mine;
+      const int n = kept + min(step, p.chunks - c0) * p.top_k;
+      for (int i = kept + threadIdx.x; i < n; i += 256) {
+        const int j = i - kept;
+        s_entry[i] = reinterpret_cast<const uint64_t*>(ws + (c0 + j / p.top_k) * chunk_bytes(p.top_k) + sizeof(ChunkStats))[j % p.top_k];
       }
+      if (threadIdx.x == 0) s_count = 0;
+      __syncthreads();
+      auto search = [&](auto groups_c) __attribute__((always_inline)) {   // by every wave for itself
+        constexpr int kGroups = decltype(groups_c)::value;
+        uint32_t key[kGroups];
+#pragma unroll
+        for (int r = 0; r < kGroups; ++r) key[r] = r * 64 + lane < n ? static_cast<uint32_t>(s_entry[r * 64 + lane] >> 32) : 0;
+        uint32_t found = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+          const uint32_t trial = found | 1u << bit;
+          int reach = 0;
+#pragma unroll
+          for (int r = 0; r < kGroups; ++r) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] >= trial));
+          if (reach >= p.top_k) found = trial;
+        }
+        return found;
+      };
+      const uint32_t found = n <= 64 ? search(std::integral_constant<int, 1>{}) : n <= 256 ? search(std::integral_constant<int, 4>{})
+                                                                                           : search(std::integral_constant<int, kSlots / 64>{});
+      for (int i = threadIdx.x; i < n; i += 256) {
+        const uint64_t mine = s_entry[i];
+        if (mine != 0 && static_cast<uint32_t>(mine >> 32) >= found) s_reach[atomicAdd(&s_count, 1)] = mine;
+      }
+      __syncthreads();
+      rank_entries(s_reach, s_count, p.top_k, s_top);
       __syncthreads();
       if (c0 + step < p.chunks) {
         for (int i = threadIdx.x; i < p.top_k; i += 256) s_entry[i] = s_top[i];
@@ -388,20 +422,24 @@ __global__ void __launch_bounds__(256) logprob_join_kernel(const LogprobParams p
   write_row<T>(p, row, m, l, t, token_logit, s_top);
 }
 
-// How a call is cut. A row that one workgroup of 1024 threads holds in registers takes one launch and is the
-// choice for few rows, where the launch is most of the time; many rows take workgroups of 512 threads with
-// half as much each, of which a CU holds four, so that the loads of some overlap the arithmetic of others.
+// How a call is cut. A workgroup of 512 threads holds 8 granules of 16 bytes per thread in registers; a CU holds four
+// such workgroups, so that the loads of some overlap the arithmetic of others. A row that fits one takes one launch. Where
+// a row is cut anyway and the pieces would leave CUs idle, a thread takes half as much: 8 rows of 50001 fp16 10.5 instead
+// of 12.1 us, one of 131072 bf16 12.4 instead of 14.9 (a quarter: 16.8, the join has more to rank). Whole rows of up to
+// 131072 in a workgroup of 1024 threads saved the second launch and lost by the longer chain: 15.8 instead of 12.6 us
+// for 104 rows of 50001.
 struct Cut {
-  bool whole_rows;
+  bool small;
   int chunks;
 };
 // `aligned`: every row starts 16-byte aligned, which is only known with the pointer; the workspace is sized without.
 Cut cut_of(const fta_logprob_args& a, bool aligned) {
   const int vec = a.dtype == FTA_F32 ? 4 : 8;
   const int64_t span = static_cast<int64_t>(a.vocab) + (aligned ? 0 : vec - 1);   // with the largest possible lead
+  const auto chunks = [vec](int64_t values, int loads) { return (values + kThreads * loads * vec - 1) / (kThreads * loads * vec); };
   Cut c;
-  c.whole_rows = a.rows <= 128 && span <= 1024 * 16 * vec;
-  c.chunks = c.whole_rows ? 1 : static_cast<int>((span + 512 * 8 * vec - 1) / (512 * 8 * vec));
+  c.small = chunks(a.vocab, 8) > 1 && a.rows * chunks(a.vocab, 4) <= 256;
+  c.chunks = static_cast<int>(chunks(span, c.small ? 4 : 8));
   return c;
 }
 
@@ -424,8 +462,9 @@ int launch(const LogprobParams& p, const Cut& cut, hipStream_t stream) {
   const int64_t grid = p.rows * p.chunks;
   if (grid > 0x7fffffffLL) return FTA_ERR_SHAPE;
   const dim3 g(static_cast<unsigned>(grid));
-  if (cut.whole_rows) return launch_checked(logprob_kernel<T, 1024, 16>, g, dim3(1024), 0, stream, p);
-  if (int st = launch_checked(logprob_kernel<T, 512, 8>, g, dim3(512), 0, stream, p)) return st;
+  if (int st = cut.small ? launch_checked(logprob_kernel<T, 4>, g, dim3(kThreads), 0, stream, p)
+                         : launch_checked(logprob_kernel<T, 8>, g, dim3(kThreads), 0, stream, p))
+    return st;
   if (cut.chunks == 1) return FTA_OK;
   return launch_checked(logprob_join_kernel<T>, dim3(static_cast<unsigned>(p.rows)), dim3(256), 0, stream, p);
 }
