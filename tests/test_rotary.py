@@ -96,6 +96,9 @@ SHAPES = [
     (2, 2, 1, 4, 128, 2, True, True, torch.float32, 0.5),         # one pair
     (1, 8, 2, 9, 256, 254, True, False, torch.float16, 1.0),
     (2, 3, 3, 2, 256, 128, False, False, torch.float32, 1.0),
+    (1, 2, 1, 3, 32, 8, False, False, torch.float32, 2.0),        # one turning unit, three that copy
+    (2, 2, 1, 3, 128, 112, False, False, torch.bfloat16, 1.0),
+    (1, 2, 2, 5, 64, 8, True, False, torch.float16, 3.0),
 ]
 
 
@@ -130,7 +133,8 @@ def test_kernel_source_on_host_threads(host_step_lib, shape):
 # ---------------------------------------------------------------- GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", SHAPES + [(2, 32, 8, 300, 128, 128, False, False, torch.bfloat16, 1.0),
-                                            (64, 40, 8, 130, 128, 96, True, False, torch.float16, 1.0)])
+                                            (64, 40, 8, 130, 128, 96, True, False, torch.float16, 1.0),
+                                            (64, 16, 4, 130, 128, 64, False, False, torch.float16, 1.0)])
 def test_matches_the_definition(shape):
     x, opt = make(shape, 1, DEV)
     for seed in (1, 2):     # the second call runs from the remembered signature
@@ -138,6 +142,15 @@ def test_matches_the_definition(shape):
         q, k = apply_rotary(x["q"], x["k"], x["positions"], x["inv_freq"], kv_seq_len=x["kv_seq_len"], **opt)
         for got, name in ((q, "q"), (k, "k")):
             check(got, x[name], rotary_oracle(x[name], x["positions"], x["inv_freq"], x["kv_seq_len"], **opt), opt["attention_factor"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_values_behind_rotary_dim_are_copied_as_they_are(interleaved):
+    q = torch.randn(2, 3, 5, 64, device=DEV).half()
+    q[..., 32:] = torch.tensor([float("nan"), float("inf"), -float("inf"), -0.0], device=DEV).half().repeat(8)
+    out, _ = apply_rotary(q, None, torch.arange(5, device=DEV), rotary_frequencies(32, device=DEV)[0], interleaved=interleaved, attention_factor=0.5)
+    assert torch.equal(out[..., 32:].view(torch.int16), q[..., 32:].view(torch.int16)) and out[..., :32].isfinite().all()
 
 
 @pytest.mark.gpu
