@@ -88,7 +88,9 @@ __device__ __forceinline__ void unrolled(F&& f) {
 }
 
 template <typename T> constexpr bool kIs32 = sizeof(T) == 4;
-template <typename T> constexpr int kTileKeys = kIs32<T> ? 32 : 64;
+// Keys of a tile; WK waves of the same 32 rows share them.
+template <typename T, int WK> constexpr int kTileKeys = kIs32<T> ? 32 * WK : 64;
+template <typename T, int D, int WK> constexpr int kLdsBytes = 4 * RowTile<D * static_cast<int>(sizeof(T)), kTileKeys<T, WK>>::kBytes;
 
 // S^T block += K fragment x Q fragment, 16 bytes of a row each: one product for 16-bit types, four for f32.
 template <typename T>
@@ -101,6 +103,21 @@ __device__ __forceinline__ f32x16 mma_chunk(u32x4 a, u32x4 b, f32x16 c) {
   } else {
     return Mfma<T>::mma(__builtin_bit_cast(typename Mfma<T>::Vec8, a), __builtin_bit_cast(typename Mfma<T>::Vec8, b), c);
   }
+}
+
+// tanh(y) for f32 calls, where the form 1 - 2 / (1 + e^(2 y)) alone would show: its error is 2^-23 absolute and a cap
+// multiplies it. Below 0.45 the series of tanh through y^13 (the next term is 2^-25 of the value), above it that form,
+// there off by at most 3.1e-7 of the value. The library's tanhf took half as long again per score.
+__device__ __forceinline__ float tanh_of(float y) {
+  const float q = y * y;
+  float series = __builtin_fmaf(q, 21844.f / 6081075.f, -1382.f / 155925.f);
+  series = __builtin_fmaf(q, series, 62.f / 2835.f);
+  series = __builtin_fmaf(q, series, -17.f / 315.f);
+  series = __builtin_fmaf(q, series, 2.f / 15.f);
+  series = __builtin_fmaf(q, series, -1.f / 3.f);
+  series = __builtin_fmaf(y * q, series, y);
+  const float far = __builtin_fmaf(-2.f, fast_rcp(1.f + fast_exp2(2.f * kLog2e * y)), 1.f);
+  return q < 0.2025f ? series : far;
 }
 
 // What a sequence contributes to the line, per unit.
@@ -197,7 +214,7 @@ template <typename T, int D, int WK, bool PAGED>
 __global__ void __launch_bounds__(256)
 FTA_WAVES_PER_EU((D <= 128 ? 2 : 1))   // head_dim 256 needs the whole register file
 shaped_kernel(const ShapedParams p) {
-  constexpr int kKeys = kTileKeys<T>;
+  constexpr int kKeys = kTileKeys<T, WK>;
   constexpr int ES = sizeof(T);
   using Tile = RowTile<D * ES, kKeys>;
   constexpr int kStages = 2;
@@ -211,7 +228,7 @@ shaped_kernel(const ShapedParams p) {
   static_assert(NB >= 1 && Tile::kBlocks % 4 == 0, "tile shape");
 
   FTA_DYNAMIC_LDS(smem);
-  __shared__ uint32_t s_seen[2];   // keys of a tree tile that a row of the workgroup sees
+  __shared__ uint32_t s_seen[kKeys / 32];   // keys of a tree tile that a row of the workgroup sees
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 31, lh = lane >> 5;
@@ -264,7 +281,7 @@ shaped_kernel(const ShapedParams p) {
   const int64_t k_lane = ((PAGED ? 0 : wave * RPB) + ld_row) * k_row + ld_chunk * 16, v_lane = ((PAGED ? 0 : wave * RPB) + ld_row) * v_row + ld_chunk * 16;
   const int64_t k_step = 4 * RPB * k_row, v_step = 4 * RPB * v_row;   // to the wave's next block
   const uint32_t lds0 = lds_address(smem);
-  const int kb0 = WK == 2 ? (wave & 1) * NB : 0;          // first key block of this wave
+  const int kb0 = wave % WK * NB;          // first key block of this wave
   const uint32_t k_rd = lds0 + Tile::at(li, lh) + kb0 * Tile::at(32, 0);
   // 16-bit V^T: 16-lane group g covers columns 16 (g % 2) .. + 15 of a 32-column block, lane s of it addresses key
   // s / 4, columns 4 (s % 4) .. + 3. f32 V: lane (i, h) reads column i of the keys 4 h + r % 4 + 8 (r / 4).
@@ -275,7 +292,7 @@ shaped_kernel(const ShapedParams p) {
   const int64_t k_page = p.k_stride[0] * ES, v_page = p.v_stride[0] * ES;
 
   // Scores in units of log2 e: without a cap z = c s; with one cap2 tanh(x / cap), the tanh written out as
-  // 1 - 2 / (1 + 2^(ex s)) (f32: taken as it is, of ex s).
+  // 1 - 2 / (1 + 2^(ex s)) (f32: tanh_of(ex s)).
   const bool capped = p.softcap > 0.f, sloped = p.slopes != nullptr;
   const float c = p.scale * kLog2e;
   const float cap2 = p.softcap * kLog2e;
@@ -418,8 +435,8 @@ shaped_kernel(const ShapedParams p) {
     auto tree_scores = [&](float (&s)[NB][16], int key0, int lane_key) __attribute__((always_inline)) {
       const auto* c = parameters_again(p);
       const int64_t mrow = b * c->mask_stride[0] + head * c->mask_stride[1] + qi * c->mask_stride[2];
-      if (c->mask_packed) {   // the keys of a tile lie in one word
-        const uint64_t word = static_cast<const uint64_t*>(c->mask)[mrow + (key0 >> 6)] >> (lane_key & 63);
+      if (c->mask_packed) {   // a wave's keys of a tile lie in one word
+        const uint64_t word = static_cast<const uint64_t*>(c->mask)[mrow + (min(lane_key, L - 1) >> 6)] >> (lane_key & 63);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -442,15 +459,14 @@ shaped_kernel(const ShapedParams p) {
           }
       }
       if (c->slopes || c->window > 0) {
-        int key_depth = min(key0 + lane % kKeys, L - 1);   // depths of the tile's keys, one per lane, handed round
+        int key_depth = min(key0 + 32 * kb0 + lane % (32 * NB), L - 1);   // depths of the wave's keys, one per lane, handed round
         if (c->depths) key_depth = max(c->depths[b * c->depth_stride + key_depth], 0);
         const int window = c->window > 0 ? c->window : 0x7fffffff;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int k0 = 32 * kb0 + key_of(nb, r);
-            const int d0 = __builtin_amdgcn_readlane(key_depth, k0), d1 = __builtin_amdgcn_readlane(key_depth, k0 + 4);
+            const int d0 = __builtin_amdgcn_readlane(key_depth, key_of(nb, r)), d1 = __builtin_amdgcn_readlane(key_depth, key_of(nb, r) + 4);
             const int away = depth - (lh ? d1 : d0);
             const float z = __builtin_fmaf(-slope, static_cast<float>(away), s[nb][r]);
             s[nb][r] = away >= window ? neg_inf() : z;
@@ -565,7 +581,7 @@ shaped_kernel(const ShapedParams p) {
             pin(s[nb][r]);
             float z;
             if constexpr (!decltype(capped_c)::value) z = __builtin_fmaf(c, s[nb][r], base);
-            else if constexpr (kIs32<T>) z = __builtin_fmaf(cap2, tanhf(ex * s[nb][r]), base);   // (the form below is 2^-23 cap off, which f32 results show)
+            else if constexpr (kIs32<T>) z = __builtin_fmaf(cap2, tanh_of(ex * s[nb][r]), base);
             else z = __builtin_fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(ex * s[nb][r])), base);
             if constexpr (decltype(sloped_c)::value) z = __builtin_fmaf(slope, static_cast<float>(key_of(nb, r)), z);
             s[nb][r] = z;
@@ -676,14 +692,14 @@ shaped_kernel(const ShapedParams p) {
       }
     }
 
-    // ---- two waves of the same rows: the upper key half's wave parks its state, the lower one's takes it in
+    // ---- waves of the same rows: those behind the first park their states, the first takes them in
     bool writes = wave_active;
-    if constexpr (WK == 2) {
+    if constexpr (WK > 1) {
       constexpr int kWords = 2 + 16 * DB;
-      static_assert(2 * kWords * 64 * 4 <= 2 * kStages * Tile::kBytes, "the parked states fit the rings");
-      float* park = reinterpret_cast<float*>(smem) + (wave >> 1) * kWords * 64 + lane;
+      static_assert(4 * kWords * 64 * 4 <= 2 * kStages * Tile::kBytes, "the parked states fit the rings");
+      float* park = reinterpret_cast<float*>(smem) + wave * kWords * 64 + lane;
       workgroup_barrier();   // the stages are done with
-      if ((wave & 1) && wave_active) {
+      if (wave % WK != 0 && wave_active) {
         park[0] = m_run;
         park[64] = l_run;
 #pragma unroll
@@ -692,17 +708,21 @@ shaped_kernel(const ShapedParams p) {
           for (int r = 0; r < 16; ++r) park[(2 + db * 16 + r) * 64] = o[db][r];
       }
       __syncthreads();
-      if (!(wave & 1) && wave_active) {
-        const float m_other = park[0], m_both = fmaxf(m_run, m_other), m_use = m_both == neg_inf() ? 0.f : m_both;
-        const float mine = fast_exp2(m_run - m_use), theirs = fast_exp2(m_other - m_use);
-        l_run = l_run * mine + park[64] * theirs;
-        m_run = m_both;
+      writes = wave_active && wave % WK == 0;
+      if (writes) {
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+        for (int w = 1; w < WK; ++w) {
+          const float* other = park + w * kWords * 64;
+          const float m_other = other[0], m_both = fmaxf(m_run, m_other), m_use = m_both == neg_inf() ? 0.f : m_both;
+          const float mine = fast_exp2(m_run - m_use), theirs = fast_exp2(m_other - m_use);
+          l_run = l_run * mine + other[64] * theirs;
+          m_run = m_both;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[db][r] = o[db][r] * mine + park[(2 + db * 16 + r) * 64] * theirs;
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[db][r] = o[db][r] * mine + other[(2 + db * 16 + r) * 64] * theirs;
+        }
       }
-      writes = wave_active && !(wave & 1);
     }
 
     // ---- the result, or a partial
@@ -759,7 +779,7 @@ shaped_kernel(const ShapedParams p) {
 // one is a round trip to memory).
 template <typename T, int D, int WK>
 __global__ void __launch_bounds__(256) shaped_join_kernel(const ShapedParams p) {
-  constexpr int kKeys = kTileKeys<T>, kRowsPerWg = 128 / WK, kRowsPerBlock = 256 / (D / 4), kTogether = 8;
+  constexpr int kKeys = kTileKeys<T, WK>, kRowsPerWg = 128 / WK, kRowsPerBlock = 256 / (D / 4), kTogether = 8;
   const int per_pair = (p.rows + kRowsPerBlock - 1) / kRowsPerBlock;
   const int pair = blockIdx.x / per_pair;
   const int unit = pair % p.units;
@@ -821,14 +841,16 @@ int cut_of(const fta_shaped_args& a, int num_cus, Cut* out) {
   if (num_cus <= 0) num_cus = kDefaultCUs;
   Cut c{};
   const bool is32 = a.dtype == FTA_F32;
-  const int keys = is32 ? 32 : 64;
   c.heads_per_unit = a.cur_heads == a.num_kv_heads ? a.num_q_heads / a.num_kv_heads : 1;
   c.units = a.num_q_heads / c.heads_per_unit;
   const int64_t rows = static_cast<int64_t>(c.heads_per_unit) * a.q_len;
   if (rows > 1 << 24) return FTA_ERR_SHAPE;
   c.rows = static_cast<int>(rows);
-  // Units of up to 64 rows: two waves per 32 rows, so that all four compute.
-  c.key_waves = !is32 && c.rows <= 64 ? 2 : 1;
+  // Units of up to 64 rows: two waves per 32 rows, so that all four compute. f32 tiles take four times the memory and
+  // eight times the matrix unit's cycles a key, and few rows leave most of the waves idle: up to 32 rows take four
+  // waves where the stages fit LDS.
+  c.key_waves = c.rows > 64 || (is32 && a.head_dim > 128) ? 1 : is32 && c.rows <= 32 && a.head_dim <= 64 ? 4 : 2;
+  const int keys = is32 ? 32 * c.key_waves : 64;
   c.rows_per_wg = 128 / c.key_waves;
   c.row_blocks = (c.rows + c.rows_per_wg - 1) / c.rows_per_wg;
   c.tree_tiles = (a.q_len + keys - 1) / keys;
@@ -838,7 +860,8 @@ int cut_of(const fta_shaped_args& a, int num_cus, Cut* out) {
   const int64_t pairs = static_cast<int64_t>(a.bsz) * c.units;
   const int64_t line = pairs * ((a.cache_len + keys - 1) / keys + 1 + static_cast<int64_t>(kTreeWeight) * c.tree_tiles);
   if (line > 0x3fffffff || pairs * c.row_blocks > 0x3fffffff) return FTA_ERR_SHAPE;
-  const int per_cu = a.head_dim <= 128 ? 2 : 1;
+  // (an f32 tile of more than 16 KiB leaves room for one workgroup)
+  const int per_cu = a.head_dim > 128 || (is32 && keys * a.head_dim > 4096) ? 1 : 2;
   c.whole = cap_tiles <= 2 * kMinStretch;
   c.groups = c.whole ? static_cast<int>(pairs) : std::max(1, num_cus * per_cu / c.row_blocks);
   c.rows_cap = std::min(c.rows, c.rows_per_wg);
@@ -896,8 +919,8 @@ int validate(const fta_shaped_args& a) {
 
 template <typename T, int D, int WK, bool PAGED>
 int launch(const ShapedParams& p, hipStream_t stream) {
-  constexpr int kSmem = 4 * RowTile<D * static_cast<int>(sizeof(T)), kTileKeys<T>>::kBytes;
-  static_assert(kSmem <= 160 * 1024 / (D <= 128 ? 2 : 1), "LDS budget");
+  constexpr int kSmem = kLdsBytes<T, D, WK>;
+  static_assert(kSmem <= 160 * 1024 / (D <= 128 && D * kTileKeys<T, WK> * sizeof(T) <= 16384 ? 2 : 1), "LDS budget");
   auto kern = shaped_kernel<T, D, WK, PAGED>;
   if (kSmem > 64 * 1024) {   // once per kernel and device
     static thread_local int configured_device = -1;
@@ -918,7 +941,10 @@ int launch(const ShapedParams& p, hipStream_t stream) {
 
 template <typename T, int D>
 int launch_d(const ShapedParams& p, const Cut& c, hipStream_t stream) {
-  if constexpr (!kIs32<T>) {
+  if constexpr (kIs32<T> && D <= 64) {
+    if (c.key_waves == 4) return p.table ? launch<T, D, 4, true>(p, stream) : launch<T, D, 4, false>(p, stream);
+  }
+  if constexpr (!kIs32<T> || D <= 128) {
     if (c.key_waves == 2) return p.table ? launch<T, D, 2, true>(p, stream) : launch<T, D, 2, false>(p, stream);
   }
   return p.table ? launch<T, D, 1, true>(p, stream) : launch<T, D, 1, false>(p, stream);

@@ -58,10 +58,10 @@ def make(seed, bsz, hq, hkv, L, D, cache, dtype, lens, page=0, cur_heads=None, d
     return {n: t.to(device) for n, t in x.items()}
 
 
-def options(hq, bsz, softcap=0.0, slopes=False, window=0, first=None, device="cpu", **kw):
+def options(hq, bsz, softcap=0.0, slopes=False, window=0, first=None, device="cpu", falling=True, **kw):
     opt = dict(softcap=softcap, window=window, **kw)
     if slopes:
-        opt["slopes"] = (2.0 ** (-8.0 * torch.arange(1, hq + 1) / hq)).to(device)
+        opt["slopes"] = (2.0 ** (-8.0 * torch.arange(1, hq + 1) / hq)).to(device) * (1.0 if falling else -1.0)
     if first is not None:
         opt["first_key"] = torch.tensor(first, dtype=torch.int32, device=device)
     return opt
@@ -78,6 +78,10 @@ CASES = {
     "paged 128, two tree tiles": ((1, 2, 1, 70, 64, 384, torch.bfloat16, [300]), dict(page=128), dict(softcap=50.0)),
     "f32": ((2, 4, 2, 6, 64, 120, torch.float32, [120, 31]), {}, dict(softcap=10.0, slopes=True)),
     "f32 paged, window, D 128": ((1, 2, 1, 35, 128, 96, torch.float32, [90]), dict(page=32), dict(window=40)),
+    "f32, 64 keys a tile": ((1, 2, 1, 25, 128, 150, torch.float32, [150]), {}, dict(softcap=30.0, slopes=True, window=101)),
+    "f32, 128 keys a tile, paged": ((2, 2, 2, 9, 32, 304, torch.float32, [300, 129]), dict(page=16), dict(softcap=4.0, first=[140, 3])),
+    "f32, 130 rows": ((1, 2, 1, 65, 32, 70, torch.float32, [70]), {}, dict(slopes=True)),
+    "rising bias, capped": ((1, 2, 1, 3, 64, 900, torch.bfloat16, [900]), {}, dict(softcap=2.0, slopes=True, falling=False)),
     "head_dim 256": ((1, 2, 1, 3, 256, 140, torch.bfloat16, [129]), {}, dict(softcap=25.0, slopes=True)),
     "f32 head_dim 256": ((1, 1, 1, 2, 256, 64, torch.float32, [50]), {}, dict(slopes=True)),
     "head_dim 32, 130 rows": ((1, 2, 1, 65, 32, 128, torch.float16, [128]), {}, dict(window=90)),
@@ -163,6 +167,12 @@ def test_kernel_source_on_host_threads(host_lib, name):
     host_lib.host_block_loads_land_late(len(name) % 2)      # half of the cases with loads that land as late as the waits allow
     check(host_call(host_lib, x, opt), oracle(x, opt), x, opt)
     host_lib.host_block_loads_land_late(0)
+
+
+@pytest.mark.parametrize("name", ["f32", "f32, 64 keys a tile", "f32, 130 rows", "paged 128, two tree tiles", "tree, slopes, two tiles of rows"])
+def test_packed_masks_on_host_threads(host_lib, name):
+    x, opt = case_inputs(name)
+    check(host_call(host_lib, {**x, "mask": pack_mask(x["mask"])}, opt), oracle(x, opt), x, opt)
 
 
 def test_rows_that_see_nothing_and_what_nobody_sees(host_lib):
