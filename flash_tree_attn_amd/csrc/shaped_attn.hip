@@ -890,7 +890,8 @@ int validate_sizes(const fta_shaped_args& a) {
     return FTA_ERR_SHAPE;
   if (a.num_q_heads % a.num_kv_heads != 0) return FTA_ERR_SHAPE;
   if (a.cur_heads != a.num_kv_heads && a.cur_heads != a.num_q_heads) return FTA_ERR_SHAPE;
-  if (!(a.softcap >= 0.f) || !std::isfinite(a.softcap) || !std::isfinite(a.sm_scale)) return FTA_ERR_UNSUPPORTED;
+  if (!(a.softcap >= 0.f) || !std::isfinite(kLog2e * a.softcap) || !std::isfinite(kLog2e * a.sm_scale)) return FTA_ERR_UNSUPPORTED;
+  if (a.softcap > 0.f && !std::isfinite(2.f * kLog2e * a.sm_scale / a.softcap)) return FTA_ERR_UNSUPPORTED;   // the tanh's argument
   return FTA_OK;
 }
 

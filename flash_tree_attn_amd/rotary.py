@@ -92,7 +92,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     dev = q.device
     if dev.type != "cuda":
         raise RuntimeError("apply_rotary runs on the GPU only; there is no CPU fallback")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, inv_freq)):
         raise RuntimeError("apply_rotary has no backward pass: call it under torch.no_grad()")
     if q.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {q.dtype}")

@@ -53,7 +53,7 @@ def shaped_tree_attention(
     dev = q.device
     if dev.type != "cuda":
         raise RuntimeError("shaped_tree_attention runs on the GPU only; there is no CPU fallback")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache, current_k, current_v)):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache, current_k, current_v, mask, slopes) if t is not None):
         raise RuntimeError("shaped_tree_attention has no backward pass: call it under torch.no_grad()")
     if q.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {q.dtype}")
@@ -125,7 +125,7 @@ def shaped_tree_attention(
         a.first_key = first_key.data_ptr()
     if depths is not None:
         a.depths, a.depth_stride = depths.data_ptr(), depths.stride(0) if depths.dim() == 2 and depths.size(0) > 1 else 0
-    a.max_seq_len_hint = 0 if max_seq_len_in_batch is None else max(int(max_seq_len_in_batch), 1)
+    a.max_seq_len_hint = 0 if max_seq_len_in_batch is None else min(max(int(max_seq_len_in_batch), 1), 0x7fffffff)
     a.dtype, a.len_dtype = _DTYPES[q.dtype], _lib.FTA_I64 if kv_seq_len.dtype == torch.int64 else _lib.FTA_I32
     a.mask_kind = _lib.MASK_PACKED_U64 if mask.dtype == torch.int64 else _lib.MASK_ADDITIVE_F32
     a.window, a.softcap, a.sm_scale = int(window), float(softcap), scale

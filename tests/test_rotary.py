@@ -188,5 +188,7 @@ def test_refusals():
             ok(**kw)
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no_grad"):
         ok(q=q.clone().requires_grad_())
+    with torch.enable_grad(), pytest.raises(RuntimeError, match="no_grad"):
+        ok(inv=inv.clone().requires_grad_())
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no_grad"):   # the same signature, remembered by now
         ok(q=q.clone().requires_grad_())

@@ -232,7 +232,7 @@ def shaped_args(**kw):
 @pytest.mark.parametrize("kw, status", [
     (dict(q=None), -1), (dict(mask=None), -1), (dict(out=None), -1), (dict(head_dim=96), -2), (dict(dtype=7), -6), (dict(len_dtype=2), -6), (dict(mask_kind=2), -6),
     (dict(bsz=0), -7), (dict(q_len=0), -7), (dict(window=-1), -7), (dict(num_q_heads=9), -7), (dict(cur_heads=4), -7), (dict(cache_len=-1), -7),
-    (dict(softcap=-1.0), -9), (dict(softcap=float("nan")), -9), (dict(softcap=float("inf")), -9), (dict(sm_scale=float("nan")), -9),
+    (dict(softcap=-1.0), -9), (dict(softcap=float("nan")), -9), (dict(softcap=float("inf")), -9), (dict(softcap=3e38), -9), (dict(softcap=1e-40), -9), (dict(sm_scale=float("nan")), -9),
     (dict(block_table=0x1000, page_size=48, block_table_stride=100), -3), (dict(block_table=0x1000, page_size=64, block_table_stride=1), -7),
     (dict(block_table=0x1000, page_size=64, block_table_stride=9, cache_len=0), -7), (dict(k_cache=0x1008), -8), (dict(mask=0x1002), -8), (dict(depth_stride=-1), -8),
 ])
@@ -398,3 +398,9 @@ def test_refusals():
             gpu_call(x, opt, output=out)
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no_grad"):
         call(dict(x, q=x["q"].clone().requires_grad_()))
+    for again in range(2):      # also where the same call without a gradient is remembered
+        with torch.enable_grad(), pytest.raises(RuntimeError, match="no_grad"):
+            call(slopes=opt["slopes"].clone().requires_grad_())
+        with torch.enable_grad(), pytest.raises(RuntimeError, match="no_grad"):
+            call(dict(x, mask=x["mask"].clone().requires_grad_()))
+        call(slopes=opt["slopes"].clone())

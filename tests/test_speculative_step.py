@@ -1,5 +1,7 @@
 """One step of speculative decoding through all of its operators: rotary positions, tree attention with shaped scores, the
 head's logits, log probabilities, the accepted path, and the append to the cache."""
+import threading
+
 import pytest
 import torch
 
@@ -117,3 +119,36 @@ def test_two_captured_steps_replay_what_eager_steps_give():
             assert all(torch.equal(s[n], eager[n]) for n in ("q", "k", "out", "logits", "targets")), turn
             assert all(torch.equal(a, b) for a, b in zip(s["scores"], eager["scores"])) and all(torch.equal(a, b) for a, b in zip(s["path"], eager["path"]))
             assert torch.equal(lens, eager_lens) and torch.equal(m.k_cache, after[0]) and torch.equal(m.v_cache, after[1])
+
+
+@pytest.mark.gpu
+def test_threads_with_streams_of_their_own():
+    """Four threads at once, each with a model and a stream: every step gives what it gives alone."""
+    g = torch.Generator().manual_seed(6)
+    tokens = torch.randint(0, VOCAB, (BSZ, L), generator=g).to(DEV)
+    models = [Model(torch.float16, 10 + i) for i in range(4)]
+    caches = [(m.k_cache.clone(), m.v_cache.clone()) for m in models]
+    alone = [m.step(tokens, torch.empty_like(m.lens)) for m in models]
+    torch.cuda.synchronize()
+    failures = []
+
+    def run(m, cache, want):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.no_grad(), torch.cuda.stream(stream):
+                for _ in range(20):
+                    m.k_cache.copy_(cache[0])
+                    m.v_cache.copy_(cache[1])
+                    s = m.step(tokens, torch.empty_like(m.lens))
+                    stream.synchronize()
+                    assert torch.equal(s["out"], want["out"]) and torch.equal(s["path"][0], want["path"][0])
+                    assert all(torch.equal(a, b) for a, b in zip(s["scores"], want["scores"]))
+        except Exception as error:
+            failures.append(error)
+
+    threads = [threading.Thread(target=run, args=a) for a in zip(models, caches, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures[0]

@@ -274,7 +274,7 @@ def test_refusals():
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no_grad"):
         token_logprobs(x.clone().requires_grad_())
     t = torch.zeros(2, 5, dtype=torch.int64, device=DEV)
-    for args, kw in (((t[0], t, t), {}), ((t, t[:, :4], t), {}), ((t, t, t[:, :4]), {}), ((t.float(), t, t), {}), ((t, t.cpu(), t), {}), ((t, t, t), dict(max_accept=0)),
+    for args, kw in (((t[0], t, t), {}), ((t, t[:, :4], t), {}), ((t, t, t[:, :4]), {}), ((t.float(), t, t), {}), ((t, t.cpu(), t), {}), ((t, t, t), dict(max_accept=0)), ((t, t, t), dict(max_accept=1 << 32)),
                      ((t, t, t), dict(len_dtype=torch.int16)), ((t[:, :0], t[:, :0], t[:, :0]), {})):
         with pytest.raises(ValueError):
             accept_tree_path(*args, **kw)
