@@ -4,7 +4,7 @@
 // One pass over the keys with a running maximum and sum. Query heads that share a cache head form a unit, their
 // rows share one K/V stream; a workgroup of four waves holds 128 rows of a unit (or 64, with two waves per 32 rows
 // that take half of the keys each) and walks over tiles of 64 keys (f32: 32) that go from memory straight into
-// LDS (global_load_lds, two stages). Per tile a wave computes
+// LDS (global_load_lds, two stages; f32 units of up to 64 rows: two or four waves per 32 rows, 64 or 128 keys a tile). Per tile a wave computes
 //     S^T = K Q^T     (32x32x16 products, lane = query row; Q stays in registers)
 //     z = shape(S), p = 2^(z - m)        (everything in units of log2 e)
 //     O^T += V^T P^T  (V^T by transposing LDS reads, P^T straight from the accumulator registers)
@@ -12,7 +12,9 @@
 // What bounds it: the stream of K and V for calls of few rows; else the vector unit. Per 32x32 scores the two
 // products take 512 cycles of the matrix unit (head_dim 128), the plain softmax about 290 cycles of the vector
 // unit and the capped one about 670 (three transcendentals a score), so two workgroups share a CU and one's
-// products run under the other's softmax.
+// products run under the other's softmax. 64 sequences of up to 32768 keys, 64 heads on 8, 16 nodes, capped and biased
+// scores: 3.85 GB in 790 to 840 us (4.6 to 4.9 TB/s of a copy's 5.1); 8 sequences of 8192 keys, 32 heads on 8, 64 nodes, the
+// same: 125 us (550 TFLOP/s of a large product's 1135), 118 us with plain scores; one token a sequence, 84 MB: 26 us.
 //
 // The work is cut evenly whatever the lengths: the (sequence, unit) pairs' tiles are laid out as one line, every
 // workgroup takes an equal stretch of it, computed by each workgroup from the lengths on the device. A pair that

@@ -12,7 +12,9 @@
 // logits) extract the k largest one by one instead.
 // Rows cut into chunks leave (m, l, t, k keys) per chunk in the workspace and a second launch joins them.
 //
-// What bounds it: the read of the logits, with about 35 vector instructions per 64 logits next to it.
+// What bounds it: the read of the logits, with about 35 vector instructions per 64 logits next to it: 512 rows of 131072
+// take 42 us in bf16 (3.2 TB/s; 32 us without alternatives, 4.2 TB/s) and 54 us in fp32 (4.9 TB/s), the large copy's rate
+// being 5.1. Few rows are two launches of about 4.5 us each.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
