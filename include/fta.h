@@ -385,9 +385,10 @@ int fta_accept_path(const fta_accept_args* args, void* hip_stream);
  *     y = softcap > 0 ? softcap * tanh(x / softcap) : x
  *     z = y - slopes[head] * (p_i - p_j)  [+ mask[i, j] for a tree key]
  * and a key is left out where p_i - p_j >= window (window > 0), a cache key also where j < first_key[b] (the
- * start of this sequence's document in its cache row). A row that sees nothing yields zeros. Cache rows that no
- * query of the call may see are not read; a value row that none of the rows of a wave (32 query rows) sees adds
- * nothing whatever it holds. Additive mask values below -2.3e38 that are not -inf count as that value.
+ * start of this sequence's document in its cache row). A row that sees nothing yields zeros. Cache rows in
+ * front of max(first_key, T_b - window + 1) and from T_b on are not read, and a tree's value row that none of a
+ * workgroup's query rows sees adds nothing whatever it holds. A NaN or an infinity in a value row that some query
+ * row sees may reach every row of the same sequence and cache head, as it does in a product with weights of 0. Additive mask values below -2.3e38 that are not -inf count as that value.
  * Everything else (shapes, strides, paged caches, mask kinds, length types) is as in fta_args, for float32 too.
  */
 typedef struct fta_shaped_args {
