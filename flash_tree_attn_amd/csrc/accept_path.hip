@@ -75,7 +75,7 @@ extern "C" int fta_accept_path(const fta_accept_args* args, void* hip_stream) {
   for (int32_t t : {a.token_dtype, a.target_dtype, a.parent_dtype, a.len_dtype})
     if (t != FTA_I32 && t != FTA_I64) return FTA_ERR_DTYPE;
   if (a.bsz <= 0 || a.q_len <= 0 || a.max_accept <= 0) return FTA_ERR_SHAPE;
-  if (a.q_len > kMaxTree) return FTA_ERR_UNSUPPORTED;
+  if (a.q_len > kMaxTree || a.max_accept > 1 << 30) return FTA_ERR_UNSUPPORTED;   // (the walk's counter is 32 bits)
   for (int i = 0; i < 2; ++i)
     if (a.token_stride[i] < 0 || a.target_stride[i] < 0 || a.parent_stride[i] < 0) return FTA_ERR_STRIDE;
   AcceptParams p{};

@@ -130,8 +130,8 @@ def accept_tree_path(tree_tokens: torch.Tensor, parents: torch.Tensor, target_to
     for name, t in (("tree_tokens", tree_tokens), ("parents", parents), ("target_tokens", target_tokens)):
         if t.dtype not in _INT_DTYPES or t.device != dev:
             raise ValueError(f"{name} must be an int32 / int64 tensor on tree_tokens' device")
-    if max_accept is not None and not 1 <= int(max_accept) < 1 << 31:
-        raise ValueError("max_accept must be at least 1 (the root)")
+    if max_accept is not None and not 1 <= int(max_accept) <= 1 << 30:
+        raise ValueError("max_accept must be between 1 (the root) and 2^30")
     if len_dtype not in _INT_DTYPES:
         raise ValueError("len_dtype must be torch.int32 or torch.int64")
     a = _lib.FtaAcceptArgs()

@@ -363,7 +363,7 @@ typedef struct fta_accept_args {
 
   int32_t bsz;
   int32_t q_len;             /* 1 .. 16384 */
-  int32_t max_accept;        /* >= 1 */
+  int32_t max_accept;        /* 1 .. 2^30 */
   int32_t token_dtype;       /* fta_len_dtype */
   int32_t target_dtype;      /* fta_len_dtype */
   int32_t parent_dtype;      /* fta_len_dtype */

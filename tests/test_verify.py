@@ -88,7 +88,7 @@ def accept_args(**kw):
 
 @pytest.mark.parametrize("kw, status", [
     (dict(tree_tokens=None), -1), (dict(next_token=None), -1), (dict(token_dtype=2), -6), (dict(len_dtype=-1), -6), (dict(bsz=0), -7), (dict(q_len=0), -7),
-    (dict(max_accept=0), -7), (dict(q_len=16385), -9),
+    (dict(max_accept=0), -7), (dict(q_len=16385), -9), (dict(max_accept=(1 << 30) + 1), -9),
 ])
 def test_accept_argument_errors(fta_lib, kw, status):
     assert fta_lib.fta_accept_path(C.byref(accept_args(**kw)), None) == status
@@ -274,7 +274,7 @@ def test_refusals():
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no_grad"):
         token_logprobs(x.clone().requires_grad_())
     t = torch.zeros(2, 5, dtype=torch.int64, device=DEV)
-    for args, kw in (((t[0], t, t), {}), ((t, t[:, :4], t), {}), ((t, t, t[:, :4]), {}), ((t.float(), t, t), {}), ((t, t.cpu(), t), {}), ((t, t, t), dict(max_accept=0)), ((t, t, t), dict(max_accept=1 << 32)),
+    for args, kw in (((t[0], t, t), {}), ((t, t[:, :4], t), {}), ((t, t, t[:, :4]), {}), ((t.float(), t, t), {}), ((t, t.cpu(), t), {}), ((t, t, t), dict(max_accept=0)), ((t, t, t), dict(max_accept=1 << 32)), ((t, t, t), dict(max_accept=(1 << 30) + 1)),
                      ((t, t, t), dict(len_dtype=torch.int16)), ((t[:, :0], t[:, :0], t[:, :0]), {})):
         with pytest.raises(ValueError):
             accept_tree_path(*args, **kw)
