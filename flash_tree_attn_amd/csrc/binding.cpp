@@ -125,6 +125,11 @@ PyObject* launch(const Entry& e, PyObject* const* args) {
     PyEval_RestoreThread(released);
     PyTuple_SET_ITEM(result.get(), 0, PyLong_FromLong(status));
     return result.release();
+  } catch (const c10::OutOfMemoryError& error) {
+    const Held torch_module(PyImport_ImportModule("torch"));
+    const Held type(torch_module ? PyObject_GetAttrString(torch_module.get(), "OutOfMemoryError") : nullptr);
+    if (type) PyErr_SetString(type.get(), error.what_without_backtrace());
+    return nullptr;
   } catch (const std::exception& error) {
     PyErr_SetString(PyExc_RuntimeError, error.what());
     return nullptr;

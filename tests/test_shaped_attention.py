@@ -301,6 +301,8 @@ LARGE = {
     "three blocks of rows": ((1, 8, 1, 50, 128, 3000, torch.float16, [2999]), {}, dict(softcap=20.0)),
     "f32 long": ((2, 8, 2, 20, 128, 3000, torch.float32, [3000, 1234]), dict(page=16), dict(softcap=30.0, slopes=True)),
     "head_dim 256, 64 nodes": ((2, 4, 2, 64, 256, 2000, torch.bfloat16, [2000, 77]), {}, dict(softcap=30.0)),
+    "uneven stretches": ((3, 16, 4, 20, 64, 40000, torch.bfloat16, [40000, 7, 33333]), {}, dict(softcap=30.0, slopes=True)),
+    "even stretches": ((4, 16, 4, 20, 64, 20000, torch.float16, [20000] * 4), dict(page=128), dict(slopes=True)),
     "head_dim 32": ((3, 16, 4, 33, 32, 5000, torch.float16, [5000, 1, 2500]), {}, dict(slopes=True)),
 }
 
