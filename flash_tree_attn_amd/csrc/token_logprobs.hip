@@ -267,10 +267,11 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobParams p
   }
 
   if (p.top_k > 0) {
-    // Where the threshold is not a number's (fewer than k logits that are) the k largest are extracted one by one.
+    // Where fewer than k groups of threads hold a finite logit, every finite one is a candidate, and of a small vocabulary
+    // every number; what is short of k even so (-inf and NaN fill up) is extracted one by one.
     const bool few = s_threshold < key_of(neg_inf());
-    const float least = value_of(max(s_threshold, key_of(neg_inf())));
-    if (!few && mine_number >= least) {
+    const float least = !few ? value_of(s_threshold) : p.vocab <= kSlots ? neg_inf() : -__FLT_MAX__;
+    if (mine_number >= least) {
       auto collect = [&](float v, int at) __attribute__((always_inline)) {
         if (!(v >= least)) return;
         const int slot = atomicAdd(&s_count, 1);
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobParams p
     }
     __syncthreads();
     const int n = s_count;
-    if (n <= kSlots && !few) {
+    if (n <= kSlots && (!few || n >= p.top_k)) {
       rank_entries(s_entry, n, p.top_k, s_top);
     } else {
       uint64_t last = ~0ull;

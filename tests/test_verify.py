@@ -115,6 +115,10 @@ LOGIT_CASES = [
     (2, 900, torch.float32, 1, 4, 1.0, "peaked"),
     (3, 600, torch.bfloat16, 1, 6, 1.0, "nan"),
     (2, 777, torch.float32, 0, 0, 1.0, "plain"),
+    (3, 153, torch.bfloat16, 1, 22, 1.0, "banned"),           # fewer groups of threads with logits than alternatives
+    (2, 400, torch.float16, 1, 60, 1.0, "plain"),
+    (2, 2000, torch.float32, 1, 30, 1.0, "nearly empty"),     # fewer finite logits than alternatives
+    (2, 5000, torch.bfloat16, 1, 12, 1.0, "one corner"),      # finite logits in few threads
 ]
 
 
@@ -131,6 +135,10 @@ def make_logits(case, seed, device="cpu"):
         x[rows - 1] = float("-inf")
     elif kind == "peaked":
         x[:, vocab // 3] = 90.0
+    elif kind == "nearly empty":
+        x[:, 7:] = float("-inf")
+    elif kind == "one corner":
+        x[:, 40:] = float("-inf")
     elif kind == "nan":
         x[0, 17] = float("nan")
     x = x.to(dtype)
