@@ -13,8 +13,8 @@
 // products take 512 cycles of the matrix unit (head_dim 128), the plain softmax about 290 cycles of the vector
 // unit and the capped one about 670 (three transcendentals a score), so two workgroups share a CU and one's
 // products run under the other's softmax. 64 sequences of up to 32768 keys, 64 heads on 8, 16 nodes, capped and biased
-// scores: 3.85 GB in 790 to 840 us (4.6 to 4.9 TB/s of a copy's 5.1); 8 sequences of 8192 keys, 32 heads on 8, 64 nodes, the
-// same: 125 us (550 TFLOP/s of a large product's 1135), 118 us with plain scores; one token a sequence, 84 MB: 26 us.
+// scores: 3.85 GB in 800 us (4.8 TB/s of a copy's 5.1); 8 sequences of 8192 keys, 32 heads on 8, 64 nodes, the same:
+// 123 us (563 TFLOP/s of a large product's 1135), 110 us with plain scores; one token of 8 sequences, 84 MB: 28 us.
 //
 // The work is cut evenly whatever the lengths: the (sequence, unit) pairs' tiles are laid out as one line, every
 // workgroup takes an equal stretch of it, computed by each workgroup from the lengths on the device. A pair that
