@@ -65,6 +65,11 @@ constexpr int kMinStretch = 4;
 
 // 2^z is 0 in 32 bits for z up to here (the smallest positive value is 2^-149).
 constexpr float kNoWeight = -150.f;
+// Scores are formed relative to a row's running maximum, which rounds them to 2^-24 of its size. Keys that a finite mask
+// (-10^4, the type's lowest value) puts out of reach may come before those that count, and a maximum of theirs would
+// swallow the scores behind it: one below this bound is not subtracted until the tile's own maximum is known. Scores of
+// their own that low (-89 in units of e) are rare, and such rows pay a rescaling per tile.
+constexpr float kLowMaximum = -128.f;
 
 // One 1 KiB block of LDS per wave-wide load: 1024 / ROW_BYTES rows, their 16-byte chunks interleaved, blocks 1024 +
 // one chunk column apart, so that both operand reads fall on distinct banks and every fragment address is a lane
@@ -585,7 +590,8 @@ shaped_kernel(const ShapedParams p) {
       // ---- z, relative to the running maximum: one multiply-add away from the products (or from the tanh), so that
       // 2^z needs no subtraction. A cache key's bias is linear in the constant part of its index.
       const bool whole_tile = !tree && key0 >= wave_lo && key0 + kKeys <= T_b;   // seen by every row of the wave
-      const float m_use = m_run == neg_inf() ? 0.f : m_run;
+      const bool low = m_run < kLowMaximum;   // (also where there is none yet)
+      const float m_use = low ? 0.f : m_run;
       const float away = static_cast<float>(pos - lane_key);
       const float base = (capped && !kIs32<T> ? cap2 : 0.f) - m_use - (tree ? 0.f : slope * away);
       auto shape = [&](auto capped_c, auto sloped_c) __attribute__((always_inline)) {
@@ -624,11 +630,11 @@ shaped_kernel(const ShapedParams p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
       // The maximum only has to keep the weights in range: it moves, and O and l are rescaled, when a row has no
-      // maximum yet or its scores pass it by more than 8 (weights up to 2^8).
-      if (wave_any(top > (m_run == neg_inf() ? neg_inf() : 8.f))) {
+      // maximum yet or a low one, or its scores pass it by more than 8 (weights up to 2^8).
+      if (wave_any(top > (low ? neg_inf() : 8.f))) {
         const float m_new = fmaxf(m_run, m_use + half_swap_max(top, lh));
         const float shift = m_new == neg_inf() ? 0.f : m_new - m_use;
-        const float a = m_run == neg_inf() ? 1.f : fast_exp2(-shift);   // (l and O are 0 where there was no maximum)
+        const float a = m_run == neg_inf() ? 1.f : fast_exp2(m_run - m_new);   // (l and O are 0 where there was no maximum)
         m_run = m_new;
         l_run *= a;
 #pragma unroll
