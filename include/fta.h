@@ -314,7 +314,8 @@ int fta_rotary(const fta_rotary_args* args, void* hip_stream);
  *     top_logprobs   = their log probabilities
  * A row whose every logit is -inf has lse = -inf, entropy 0 and log probabilities of -inf. A NaN or +inf in a
  * row makes its lse, entropy and log probabilities NaN (among the alternatives NaN counts as less than
- * -inf). All sums in 32 bits; outputs are float32 / int64.
+ * -inf). All sums in 32 bits; outputs are float32 / int64 (of a logit of -3e38 over a temperature below 1, or a
+ * temperature of 1e-38, lse and log probabilities are infinities of that type, not NaN).
  */
 typedef struct fta_logprob_args {
   const void* logits;        /* [rows, vocab], row stride logits_stride, inner stride 1, any alignment of its type */
