@@ -470,7 +470,7 @@ int validate_sizes(const fta_logprob_args& a) {
   if (a.id_dtype != FTA_I32 && a.id_dtype != FTA_I64) return FTA_ERR_DTYPE;
   if (a.rows <= 0 || a.vocab <= 0 || a.num_ids < 0 || a.top_k < 0 || a.top_k > a.vocab) return FTA_ERR_SHAPE;
   if (a.top_k > kMaxTop || a.vocab > 1 << 30) return FTA_ERR_UNSUPPORTED;
-  if (!(a.inv_temperature > 0.f) || !std::isfinite(a.inv_temperature)) return FTA_ERR_UNSUPPORTED;
+  if (!(a.inv_temperature > 0.f) || !std::isfinite(kLog2e * a.inv_temperature)) return FTA_ERR_UNSUPPORTED;   // the exponents' scale
   return FTA_OK;
 }
 

@@ -334,7 +334,7 @@ typedef struct fta_logprob_args {
   int32_t top_k;             /* 0 .. min(vocab, 128) */
   int32_t dtype;             /* fta_dtype of logits */
   int32_t id_dtype;          /* fta_len_dtype of token_ids */
-  float inv_temperature;     /* > 0 */
+  float inv_temperature;     /* > 0, at most 2.3e38 */
   int64_t logits_stride;
   int64_t id_stride[2];      /* row, column of token_ids */
 } fta_logprob_args;

@@ -102,6 +102,19 @@ def test_temperatures_near_zero_on_host_threads(host_step_lib, rows, vocab, dtyp
     check(host_call(host_step_lib, x, ids, 3, temperature), x, ids, 3, temperature)
 
 
+@pytest.mark.parametrize("inv_temperature, status", [(1.0, 0), (2.3e38, 0), (2.4e38, -9), (3.4e38, -9), (1e-44, 0)])
+def test_a_temperature_whose_inverse_in_units_of_log2_e_does_not_fit_is_refused(fta_lib, inv_temperature, status):
+    a = _lib.FtaLogprobArgs()
+    a.rows, a.vocab, a.logits_stride, a.dtype, a.id_dtype, a.inv_temperature = 1, 10, 10, _lib.FTA_F32, _lib.FTA_I64, inv_temperature
+    assert fta_lib.fta_logprobs_workspace(C.byref(a), C.byref(C.c_int64())) == status
+
+
+@pytest.mark.parametrize("temperature", [4.4e-39, 1e38])
+def test_the_least_and_largest_temperatures_on_host_threads(host_step_lib, temperature):  # noqa: F811
+    x, ids = logits(3, 500, torch.float32, 2)
+    check(host_call(host_step_lib, x, ids, 3, temperature), x, ids, 3, temperature)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows, vocab, dtype", COLD + [(300, 50001, torch.bfloat16), (70, 131072, torch.float32)])
 def test_temperatures_near_zero(rows, vocab, dtype):
