@@ -202,13 +202,14 @@ __device__ __forceinline__ Place place_of(const ShapedParams& p, bool by_sequenc
 // How the line is cut: into stretches whose bounds are rounded multiples of an unrounded length, so that equally long
 // pairs are cut alike (multiples of a rounded length drift and leave pieces of a tile or two, each a prologue and a
 // partial: 240 against 222 us for 16 sequences of 16384 keys, 64 heads on 8, 16 nodes). `heads` of them share the line up
-// to `middle`, the rest what is behind it. In 32-bit floats, a division each: any bounds do that both kernels agree on.
+// to `middle`, the rest what is behind it. In 32-bit floats, a division each: any bounds do that both kernels agree on, so
+// the one product with a sum behind it is written as a fused one, and no compilation rounds it differently.
 struct Stretches {
   int total, groups, heads, middle;
   float lead, tail;   // lengths
   __device__ __forceinline__ int start(int g) const {
-    const float at = g < heads ? static_cast<float>(g) * lead : static_cast<float>(g - heads) * tail;
-    const int x = static_cast<int>(at + 0.03125f);   // (a length of 43 2/3 times 3 is 131, not 130)
+    const float nth = static_cast<float>(g < heads ? g : g - heads), length = g < heads ? lead : tail;
+    const int x = static_cast<int>(__builtin_fmaf(nth, length, 0.03125f));   // (a length of 43 2/3 times 3 is 131, not 130)
     return g >= groups ? total : g < heads ? min(x, middle) : min(middle + x, total);
   }
   __device__ __forceinline__ int holder(int x) const {
