@@ -112,9 +112,11 @@ __device__ __forceinline__ f32x16 mma_chunk(u32x4 a, u32x4 b, f32x16 c) {
   }
 }
 
-// tanh(y) for f32 calls, where the form 1 - 2 / (1 + e^(2 y)) alone would show: its error is 2^-23 absolute and a cap
-// multiplies it. Below 0.45 the series of tanh through y^13 (the next term is 2^-25 of the value), above it that form,
+// tanh(y) where the form 1 - 2 / (1 + e^(2 y)) alone would show: its error is about 2^-23 absolute and a cap multiplies it.
+// f32 calls take this one, 16-bit calls under a cap above kShortCap, where that error passes 2^-13, a quarter of fp16's
+// half step (a cap of 10^6 was off by 0.02 in the output, one of 10^8 averaged all values). Below 0.45 the series of tanh through y^13 (the next term is 2^-25 of the value), above it that form,
 // there off by at most 3.1e-7 of the value. The library's tanhf took half as long again per score.
+constexpr float kShortCap = 256.f;
 __device__ __forceinline__ float tanh_of(float y) {
   const float q = y * y;
   float series = __builtin_fmaf(q, 21844.f / 6081075.f, -1382.f / 155925.f);
@@ -313,11 +315,12 @@ shaped_kernel(const ShapedParams p) {
   const int64_t k_page = p.k_stride[0] * ES, v_page = p.v_stride[0] * ES;
 
   // Scores in units of log2 e: without a cap z = c s; with one cap2 tanh(x / cap), the tanh written out as
-  // 1 - 2 / (1 + 2^(ex s)) (f32: tanh_of(ex s)).
+  // 1 - 2 / (1 + 2^(ex s)), or tanh_of(ex s).
   const bool capped = p.softcap > 0.f, sloped = p.slopes != nullptr;
+  const bool series = kIs32<T> || p.softcap > kShortCap;
   const float c = p.scale * kLog2e;
   const float cap2 = p.softcap * kLog2e;
-  const float ex = capped ? (kIs32<T> ? 1.f : 2.f * kLog2e) * p.scale / p.softcap : 0.f;
+  const float ex = capped ? (series ? 1.f : 2.f * kLog2e) * p.scale / p.softcap : 0.f;
 
   for (;;) {
     // ---- one pair: places [from, to) of its stretch
@@ -594,25 +597,32 @@ shaped_kernel(const ShapedParams p) {
       const bool low = m_run < kLowMaximum;   // (also where there is none yet)
       const float m_use = low ? 0.f : m_run;
       const float away = static_cast<float>(pos - lane_key);
-      const float base = (capped && !kIs32<T> ? cap2 : 0.f) - m_use - (tree ? 0.f : slope * away);
-      auto shape = [&](auto capped_c, auto sloped_c) __attribute__((always_inline)) {
+      const float base = (capped && !series ? cap2 : 0.f) - m_use - (tree ? 0.f : slope * away);
+      constexpr int kPlain = 0, kShort = 1, kSeries = 2;
+      auto shape = [&](auto cap_c, auto sloped_c) __attribute__((always_inline)) {
+        constexpr int kCap = decltype(cap_c)::value;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             pin(s[nb][r]);
             float z;
-            if constexpr (!decltype(capped_c)::value) z = __builtin_fmaf(c, s[nb][r], base);
-            else if constexpr (kIs32<T>) z = __builtin_fmaf(cap2, tanh_of(ex * s[nb][r]), base);
+            if constexpr (kCap == kPlain) z = __builtin_fmaf(c, s[nb][r], base);
+            else if constexpr (kCap == kSeries) z = __builtin_fmaf(cap2, tanh_of(ex * s[nb][r]), base);
             else z = __builtin_fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(ex * s[nb][r])), base);
             if constexpr (decltype(sloped_c)::value) z = __builtin_fmaf(slope, static_cast<float>(key_of(nb, r)), z);
             s[nb][r] = z;
           }
       };
-      if (capped) {
-        if (sloped && !tree) shape(std::true_type{}, std::true_type{}); else shape(std::true_type{}, std::false_type{});
+      auto shape_with = [&](auto cap_c) __attribute__((always_inline)) {
+        if (sloped && !tree) shape(cap_c, std::true_type{}); else shape(cap_c, std::false_type{});
+      };
+      if (!capped) {
+        shape_with(std::integral_constant<int, kPlain>{});
+      } else if (series) {
+        shape_with(std::integral_constant<int, kSeries>{});
       } else {
-        if (sloped && !tree) shape(std::false_type{}, std::true_type{}); else shape(std::false_type{}, std::false_type{});
+        if constexpr (!kIs32<T>) shape_with(std::integral_constant<int, kShort>{});
       }
       if (tree) {
         tree_scores(s, key0, lane_key);

@@ -1,5 +1,5 @@
 """Shaped tree attention at the ends of what its arguments may be (the kernel's source on host threads, and on the GPU):
-finite masks, from soft ones to the type's lowest value, in front of keys that count."""
+finite masks, from soft ones to the type's lowest value, in front of keys that count; caps that bind hardly or not at all."""
 import pytest
 import torch
 
@@ -45,3 +45,34 @@ def test_keys_behind_finite_masks(name):
         x["mask"] = x["mask"].masked_fill(x["mask"] == value, float("-inf"))
         if value < -1e5:      # such a key weighs nothing next to any other
             check(got, oracle(x, opt), x, opt)
+
+
+# softcap, (bsz hq hkv L D cache dtype lens), options()
+CAPPED = [(cap, shape, opt) for cap in (200.0, 300.0, 1e3, 1e5, 1e8, 2e38) for shape, opt in (
+    ((1, 2, 1, 5, 64, 130, torch.float16, [130]), {}),
+    ((1, 2, 1, 40, 64, 100, torch.bfloat16, [100]), dict(slopes=True)),
+    ((1, 2, 1, 3, 32, 100, torch.float32, [97]), {}),
+)]
+
+
+def check_capped(got, x, opt):
+    """`check`, with a cap that large counted as the scores are: |cap tanh(x / cap)| <= |x|, and no step of the arithmetic may
+    be larger than what it gives. The scores are up to 20: 16-bit calls may put 2^-21 of a cap up to 256 into an exponent
+    (under 2^-13, a quarter of fp16's half step of the weights, which `check` counts twice over)."""
+    check(got, oracle(x, opt), x, dict(opt, softcap=min(opt["softcap"], 20.0)))
+
+
+@pytest.mark.parametrize("cap, shape, opt", CAPPED)
+def test_large_caps_on_host_threads(host_lib, cap, shape, opt):  # noqa: F811
+    x = make(7, *shape)
+    x["q"] = x["q"] * 3
+    opt = options(shape[1], shape[0], softcap=cap, **opt)
+    check_capped(host_call(host_lib, x, opt), x, opt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap, shape, opt", CAPPED + [(c, (2, 8, 2, 64, 128, 2000, t, [2000, 1500]), {}) for c in (255.0, 257.0, 1e6) for t in (torch.float16, torch.bfloat16)])
+def test_large_caps(cap, shape, opt):
+    x = make(7, *shape, device=DEV)
+    opt = options(shape[1], shape[0], softcap=cap, device=DEV, **opt)
+    check_capped(gpu_call(x, opt), x, opt)
