@@ -15,6 +15,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -44,11 +45,11 @@ struct Entry {
 
 void append(std::string& key, const void* data, size_t n) { key.append(static_cast<const char*>(data), n); }
 
-// False for an argument that has no place in a signature.
-bool sign(PyObject* arg, std::string& key) {
+// False for an argument that has no place in a signature. tangents: tensors may carry some (a forward-mode level is live).
+bool sign(PyObject* arg, std::string& key, bool tangents) {
   if (THPVariable_Check(arg)) {
     const at::Tensor& t = THPVariable_Unpack(arg);
-    if (t.layout() != at::kStrided || !t.has_storage()) return false;
+    if (t.layout() != at::kStrided || !t.has_storage() || (tangents && t._fw_grad(0).defined())) return false;   // (a tangent: refused by the full checks)
     const auto sizes = t.sizes(), strides = t.strides();
     const char head[6] = {'t', static_cast<char>(t.scalar_type()), static_cast<char>(t.device().type()), static_cast<char>(t.device().index()),
                           static_cast<char>(sizes.size()), static_cast<char>(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15)};
@@ -147,8 +148,9 @@ PyObject* recall(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   std::string key;
   key.reserve(512);
   try {
+    const bool tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;   // (there is one level at most)
     for (Py_ssize_t i = 0; i < argc - 1; ++i)
-      if (!sign(args[i], key)) Py_RETURN_NONE;
+      if (!sign(args[i], key, tangents)) Py_RETURN_NONE;
   } catch (const std::exception&) {   // a tensor without memory of its own: the full checks have the say
     Py_RETURN_NONE;
   }

@@ -25,6 +25,7 @@ import threading
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -336,6 +337,15 @@ class _FastEntry:
 
 def _sig(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _refuse_derivatives(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """For the operators without derivatives: rather an error than a gradient or a tangent that is dropped."""
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise RuntimeError(f"{name} has no forward-mode derivative: pass tensors without tangents")
 
 
 def _calls() -> dict:

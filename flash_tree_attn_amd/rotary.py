@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .flash_decoding import _DTYPES, _as_rows, _calls, _check, _current_stream, _remember_call, _rows_ok
+from .flash_decoding import _DTYPES, _as_rows, _calls, _check, _current_stream, _refuse_derivatives, _remember_call, _rows_ok
 
 _INT_DTYPES = {torch.int32: _lib.FTA_I32, torch.int64: _lib.FTA_I64}
 
@@ -92,8 +92,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     dev = q.device
     if dev.type != "cuda":
         raise RuntimeError("apply_rotary runs on the GPU only; there is no CPU fallback")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, inv_freq)):
-        raise RuntimeError("apply_rotary has no backward pass: call it under torch.no_grad()")
+    _refuse_derivatives("apply_rotary", q, k, inv_freq)
     if q.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {q.dtype}")
     bsz, hq, L, D = q.shape

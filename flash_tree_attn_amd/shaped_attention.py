@@ -13,8 +13,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .flash_decoding import (_DTYPES, FtaAssertionError, _as_rows, _calls, _check, _current_stream, _num_cus, _prepare_mask, _remember_call,
-                             _rows_ok)
+from .flash_decoding import (_DTYPES, FtaAssertionError, _as_rows, _calls, _check, _current_stream, _num_cus, _prepare_mask,
+                             _refuse_derivatives, _remember_call, _rows_ok)
 
 
 def shaped_tree_attention(
@@ -53,8 +53,7 @@ def shaped_tree_attention(
     dev = q.device
     if dev.type != "cuda":
         raise RuntimeError("shaped_tree_attention runs on the GPU only; there is no CPU fallback")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache, current_k, current_v, mask, slopes) if t is not None):
-        raise RuntimeError("shaped_tree_attention has no backward pass: call it under torch.no_grad()")
+    _refuse_derivatives("shaped_tree_attention", q, k_cache, v_cache, current_k, current_v, mask, slopes)
     if q.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {q.dtype}")
     paged = block_tables is not None

@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from .flash_decoding import _DTYPES, _calls, _check, _current_stream, _remember_call
+from .flash_decoding import _DTYPES, _calls, _check, _current_stream, _refuse_derivatives, _remember_call
 
 _INT_DTYPES = {torch.int32: _lib.FTA_I32, torch.int64: _lib.FTA_I64}
 MAX_TOP_K = 128
@@ -56,8 +56,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
     dev = logits.device
     if dev.type != "cuda":
         raise RuntimeError("token_logprobs runs on the GPU only; there is no CPU fallback")
-    if torch.is_grad_enabled() and logits.requires_grad:
-        raise RuntimeError("token_logprobs has no backward pass: call it under torch.no_grad()")
+    _refuse_derivatives("token_logprobs", logits)
     if logits.dim() < 1 or logits.dtype not in _DTYPES or logits.numel() == 0:
         raise ValueError("logits must be a non-empty fp32, fp16 or bf16 tensor [..., vocab]")
     vocab = logits.size(-1)
