@@ -95,6 +95,11 @@ __device__ __forceinline__ void unrolled(F&& f) {
 }
 
 template <typename T> constexpr bool kIs32 = sizeof(T) == 4;
+// Weights are taken against a reference this far below the running maximum, in units of log2. fp16 ends at 2^-24 and
+// 2^16: with 2^7 for the largest key (up to 2^15 until the maximum moves) what is lost of 131072 keys far below it is less
+// than 2^-15 of the sum; against the maximum itself it was up to 2^-8. The other types have the range of 32 bits.
+template <typename T> constexpr float kHeadroom = 0.f;
+template <> constexpr float kHeadroom<_Float16> = 7.f;
 // Keys of a tile; WK waves of the same 32 rows share them.
 template <typename T, int WK> constexpr int kTileKeys = kIs32<T> ? 32 * WK : 64;
 template <typename T, int D, int WK> constexpr int kLdsBytes = 4 * RowTile<D * static_cast<int>(sizeof(T)), kTileKeys<T, WK>>::kBytes;
@@ -640,10 +645,10 @@ shaped_kernel(const ShapedParams p) {
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
-      // The maximum only has to keep the weights in range: it moves, and O and l are rescaled, when a row has no
-      // maximum yet or a low one, or its scores pass it by more than 8 (weights up to 2^8).
-      if (wave_any(top > (low ? neg_inf() : 8.f))) {
-        const float m_new = fmaxf(m_run, m_use + half_swap_max(top, lh));
+      // The maximum (less the headroom) only has to keep the weights in range: it moves, and O and l are rescaled, when a
+      // row has none yet or a low one, or its scores pass it by more than 8 (weights up to 2^8 times the headroom's).
+      if (wave_any(top > (low ? neg_inf() : 8.f + kHeadroom<T>))) {
+        const float m_new = fmaxf(m_run, m_use + half_swap_max(top, lh) - kHeadroom<T>);
         const float shift = m_new == neg_inf() ? 0.f : m_new - m_use;
         const float a = m_run == neg_inf() ? 1.f : fast_exp2(m_run - m_new);   // (l and O are 0 where there was no maximum)
         m_run = m_new;

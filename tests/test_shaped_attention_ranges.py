@@ -1,5 +1,6 @@
 """Shaped tree attention at the ends of what its arguments may be (the kernel's source on host threads, and on the GPU):
-finite masks, from soft ones to the type's lowest value, in front of keys that count; caps that bind hardly or not at all."""
+finite masks, from soft ones to the type's lowest value, in front of keys that count; caps that bind hardly or not at all;
+many keys far below the one that leads."""
 import pytest
 import torch
 
@@ -76,3 +77,61 @@ def test_large_caps(cap, shape, opt):
     x = make(7, *shape, device=DEV)
     opt = options(shape[1], shape[0], softcap=cap, device=DEV, **opt)
     check_capped(gpu_call(x, opt), x, opt)
+
+
+def far_below(keys, dtype, below, device="cpu"):
+    """One token whose own key leads and `keys` cached ones whose scores are `below` lower; their values differ from its."""
+    D = 64
+    x = make(9, 1, 1, 1, 1, D, keys, dtype, [keys], device=device)
+    x["q"].zero_()[..., 0] = 8.0      # times the scale of 1 / 8: the scores are the keys' first values
+    x["k_cache"][..., 0], x["current_k"][..., 0] = -below, 0.0
+    x["v_cache"].fill_(1.0)
+    x["current_v"].fill_(-1.0)
+    return x, {}
+
+
+# In units of log2 e the scores are 14.4, 25.07 and 27.4 lower: of fp16's weights the last two are below its least number, 2^-24,
+# next to a leading weight of 1. All of them together move the result by up to 2 keys e^-below.
+FAR = [(torch.float16, 10.0), (torch.float16, 17.375), (torch.float16, 19.0), (torch.bfloat16, 17.375), (torch.float32, 17.375)]
+
+
+class OneStretch:
+    """The library with a bound of the lengths that does not hold: one workgroup walks over all of a sequence's keys, as in a
+    batch that gives every one its own."""
+
+    def __init__(self, lib):
+        self.lib = lib
+
+    def fta_shaped_workspace(self, a, cus, need):
+        a._obj.max_seq_len_hint = 1
+        return self.lib.fta_shaped_workspace(a, cus, need)
+
+    def fta_shaped_decode(self, a, stream):
+        return self.lib.fta_shaped_decode(a, stream)
+
+
+@pytest.mark.parametrize("dtype, below", FAR[1:2])
+def test_many_keys_far_below_on_host_threads(host_lib, dtype, below):  # noqa: F811
+    x, opt = far_below(60000, dtype, below)
+    check(host_call(OneStretch(host_lib), x, opt), oracle(x, opt), x, opt)
+
+
+def check_far(got, x, keys):
+    """`check` in 16 bits. In 32, what bounds such a row are the sums: each addition to O or l rounds by up to 2^-24 of what is
+    there, at most l max |v| and l with max |v| = 1, a product adds two keys at a time and a wave at most every key: keys / 2
+    additions in a row for either, keys * 2^-24 of the result, and next to it the exponents' 2^-23 (score + bound of the
+    score's own sum) < 2^-23 * 200 (scores below 20 from products of up to 8 * 20) on values that differ by 2."""
+    if got.dtype != torch.float32:
+        check(got, oracle(x, {}), x, {})
+    else:
+        assert float((got.double() - oracle(x, {})).abs().max()) <= keys * 2.0 ** -24 + 2 * 200 * 2.0 ** -23
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, below", FAR)
+def test_many_keys_far_below(dtype, below):
+    for keys in (30000, 131072, 1000000):
+        x, opt = far_below(keys, dtype, below, DEV)
+        check_far(gpu_call(x, opt), x, keys)
+        if keys < 1000000:
+            check_far(gpu_call(x, opt, max_seq_len_in_batch=1), x, keys)
