@@ -155,6 +155,7 @@ int validate(const fta_rotary_args& a) {
   if (a.head_dim != 32 && a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return FTA_ERR_HEAD_DIM;
   if (a.bsz <= 0 || a.num_q_heads <= 0 || a.q_len <= 0 || a.rotary_dim < 2 || a.rotary_dim > a.head_dim || a.rotary_dim % 2) return FTA_ERR_SHAPE;
   if (a.k ? a.num_kv_heads <= 0 : a.num_kv_heads != 0) return FTA_ERR_SHAPE;
+  if (!std::isfinite(a.attention_factor)) return FTA_ERR_UNSUPPORTED;   // (also a double that left 32 bits on its way here)
   const int vec = a.dtype == FTA_F32 ? 4 : 8;
   const int64_t* strides[] = {a.q_stride, a.out_q_stride, a.k_stride, a.out_k_stride};
   const void* ptrs[] = {a.q, a.out_q, a.k, a.out_k};

@@ -292,7 +292,7 @@ typedef struct fta_rotary_args {
   int32_t freq_is_f64;
   int32_t interleaved;
   int32_t inverse;
-  float attention_factor;
+  float attention_factor;    /* finite */
   int32_t reserved;
 
   int64_t q_stride[3];       /* batch, head, row */
