@@ -60,6 +60,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
     if logits.dim() < 1 or logits.dtype not in _DTYPES or logits.numel() == 0:
         raise ValueError("logits must be a non-empty fp32, fp16 or bf16 tensor [..., vocab]")
     vocab = logits.size(-1)
+    if vocab > 1 << 30:
+        raise ValueError("a row may hold up to 2^30 logits")
     top_k = int(top_k)
     if not 0 <= top_k <= min(vocab, MAX_TOP_K):
         raise ValueError(f"top_k {top_k} is not between 0 and min(vocab, {MAX_TOP_K})")

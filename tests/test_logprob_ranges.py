@@ -131,3 +131,10 @@ def test_banned_with_the_lowest_value(vocab, dtype):
             x, ids = banned(vocab, dtype, 1, DEV)
             x, ids = x.repeat(rows, 1), ids.repeat(rows, 1)
             check(token_logprobs(x, ids, top_k=9, temperature=temperature), x, ids, 9, temperature)
+
+
+@pytest.mark.gpu
+def test_rows_of_more_logits_than_an_int_counts_are_refused():
+    for vocab in ((1 << 30) + 1, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="2\\^30"):
+            token_logprobs(torch.zeros(1, 1, device=DEV, dtype=torch.bfloat16).expand(1, vocab))
