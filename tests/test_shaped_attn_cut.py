@@ -53,7 +53,7 @@ def test_bounds_do_not_depend_on_what_the_compiler_fuses(tmp_path):
         pytest.skip("no fused multiply-add on this machine")
     text = open(os.path.join(fta_build.CSRC, "shaped_attn.hip")).read()
     start = text.index("struct Stretches {")
-    end = text.index("template <typename T, int D, int WK, bool PAGED>", start)
+    end = text.index("\n}\n", text.index(" cut_line(", start)) + 3
     src = tmp_path / "cut.cpp"
     src.write_text(PROGRAM % text[start:end])
     results = []
