@@ -2,9 +2,10 @@
 //
 // One workgroup per sequence. In parallel over the nodes: node i matches if its token is what the model picked
 // after its parent; the lowest matching child of every parent is kept with an integer minimum in LDS (the same
-// result in any order). Then every wave follows root -> first[root] -> ... through LDS, and lane k keeps the
-// k-th node. Parents precede children, so the walk ends. What bounds it: launch latency, and on long paths the
-// walk, one LDS round trip per accepted node: 2.2 us for a tree of 26 nodes, 5.0 us for 256 of 256, the kernel alone.
+// result in any order). Then the first wave follows root -> first[root] -> ... through LDS, the walk the same in all
+// of its lanes, and lane k keeps the k-th node. Parents precede children, so the walk ends. What bounds it: launch
+// latency, and on long paths the walk, one LDS round trip per accepted node: 2.2 us for a tree of 26 nodes, 5.0 us for 256
+// of 256, the kernel alone.
 #include <hip/hip_runtime.h>
 
 #include "fta_device.h"

@@ -5,8 +5,9 @@
 // second pair members; interleaved: 16 bytes of whole pairs), takes the sines of its pairs once and walks over
 // `heads_per_thread` heads with them, so that the 64-bit angles and the sines (about 60 instructions a pair)
 // are shared between heads. Units behind rotary_dim copy. Rotary dims that do not fill 16-byte units take one
-// pair per thread. What bounds it: every row read and written once (336 MB in 66 us, 5.1 TB/s);
-// calls of a few rows are launch-bound (3.2 us).
+// pair per thread. What bounds it: every row read and written once (336 MB in 73 us, 4.6 TB/s of a copy's 5.1; 66 us
+// where the inputs' 168 MB are still in the memory-side cache); calls of a few rows are launch-bound (3.3 us). Pair by
+// pair, in accesses of 2 or 4 bytes, rotary dims of 22 or 40 take 113 to 124 us for the same rows in 16 bits.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -242,7 +243,8 @@ extern "C" int fta_rotary(const fta_rotary_args* args, void* hip_stream) {
   for (int t = 0; t < 2; ++t) p.chunks[t] = (p.heads[t] + p.heads_per_thread - 1) / p.heads_per_thread;
 
   // Results that the L2s (32 MiB) cannot hold until they are read would only push the inputs out: 84 us became 78 by the
-  // alike units and 66 by these stores for 8 x 2048 rows, 32 + 8 heads of 128 values (336 MB at 5.1 TB/s, a copy's rate).
+  // alike units and 66 by these stores for 8 x 2048 rows, 32 + 8 heads of 128 values, one set of inputs again and again (its
+  // 168 MB stay in the memory-side cache; from sets in turn 73).
   const bool past_l2 = static_cast<int64_t>(a.bsz) * a.q_len * (a.num_q_heads + a.num_kv_heads) * a.head_dim * es > (int64_t{32} << 20);
 
   const int64_t threads = p.items * (p.chunks[0] + p.chunks[1]);

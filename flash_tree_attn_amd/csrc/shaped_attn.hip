@@ -13,8 +13,9 @@
 // products take 512 cycles of the matrix unit (head_dim 128), the plain softmax about 290 cycles of the vector
 // unit and the capped one about 670 (three transcendentals a score), so two workgroups share a CU and one's
 // products run under the other's softmax. 64 sequences of up to 32768 keys, 64 heads on 8, 16 nodes, capped and biased
-// scores: 3.85 GB in 800 us (4.8 TB/s of a copy's 5.1); 8 sequences of 8192 keys, 32 heads on 8, 64 nodes, the same:
-// 123 us (563 TFLOP/s of a large product's 1135), 110 us with plain scores; one token of 8 sequences, 84 MB: 28 us.
+// scores: 3.85 GB in 804 us (4.8 TB/s of a copy's 5.1); 8 sequences of 8192 keys, 32 heads on 8, 64 nodes, capped
+// scores: 124 us (558 TFLOP/s of a large product's 1135), with a bias too about as long (119 to 126, in turn with the
+// former's 120 to 127), 107 to 112 us with plain scores; one token of 8 sequences, 84 MB: 28 us.
 //
 // The work is cut evenly whatever the lengths: the (sequence, unit) pairs' tiles are laid out as one line, every
 // workgroup takes an equal stretch of it, computed by each workgroup from the lengths on the device. A pair that
@@ -700,7 +701,11 @@ shaped_kernel(const ShapedParams p) {
           for (int e = 0; e < 8; e += 2) {
             const f32x2 pair = {s[kk / 2][kk % 2 * 8 + e], s[kk / 2][kk % 2 * 8 + e + 1]};
             const auto rounded = __builtin_convertvector(pair, typename M::Vec2);
-            l_run = M::add_pair(rounded, l_run);   // l sums the rounded weights, the ones the product applies
+            // The weights enter the product in the type, as the values do: half a step each, which with l summing the
+            // rounded ones moves the result by about as much as its own rounding does (0.0023 from the 64-bit result in
+            // bf16, relative to its size, where rounding that result once is 0.0017). A second product of what they lose
+            // would double the matrix unit's share of this half.
+            l_run = M::add_pair(rounded, l_run);
             pf[kk][e] = rounded[0];
             pf[kk][e + 1] = rounded[1];
           }

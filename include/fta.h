@@ -389,7 +389,9 @@ int fta_accept_path(const fta_accept_args* args, void* hip_stream);
  * start of this sequence's document in its cache row). A row that sees nothing yields zeros. Cache rows in
  * front of max(first_key, T_b - window + 1) and from T_b on are not read, and a tree's value row that none of a
  * workgroup's query rows sees adds nothing whatever it holds. A NaN or an infinity in a value row that some query
- * row sees may reach every row of the same sequence and cache head, as it does in a product with weights of 0. Additive mask values below -2.3e38 that are not -inf count as that value.
+ * row sees may reach every row of the same sequence and cache head, as it does in a product with weights of 0.
+ * Additive mask values below -2.3e38 that are not -inf count as that value. Scores, softmax statistics and sums are
+ * held in 32 bits; in 16-bit calls the weights enter the second product in the type, as in fta_decode.
  * Everything else (shapes, strides, paged caches, mask kinds, length types) is as in fta_args, for float32 too.
  */
 typedef struct fta_shaped_args {

@@ -8,6 +8,7 @@ from flash_tree_attn_amd import _lib, apply_rotary, rotary_frequencies, shaped_t
 from flash_tree_attn_amd.flash_decoding import _refuse_derivatives
 
 DEV = "cuda"
+pytestmark = pytest.mark.filterwarnings("ignore::DeprecationWarning")      # torch's own, at the first tangent
 
 
 def test_tensors_with_tangents_have_no_signature():
