@@ -14,7 +14,7 @@
 // unit and the capped one about 670 (three transcendentals a score), so two workgroups share a CU and one's
 // products run under the other's softmax. 64 sequences of up to 32768 keys, 64 heads on 8, 16 nodes, capped and biased
 // scores: 3.85 GB in 804 us (4.8 TB/s of a copy's 5.1); 8 sequences of 8192 keys, 32 heads on 8, 64 nodes, capped
-// scores: 124 us (558 TFLOP/s of a large product's 1135), with a bias too about as long (119 to 126, in turn with the
+// scores: 124 to 127 us (558 TFLOP/s of a large product's 1135), with a bias too about as long (119 to 126, in turn with the
 // former's 120 to 127), 107 to 112 us with plain scores; one token of 8 sequences, 84 MB: 28 us.
 //
 // The work is cut evenly whatever the lengths: the (sequence, unit) pairs' tiles are laid out as one line, every
